@@ -47,6 +47,10 @@ EXPORTS = (
     "dsa_sparse_mla_fwd_fp8",
     "dsa_indexer_workspace_bytes",
     "dsa_indexer_topk",
+    "dsa_rotary",
+    "dsa_plan_pages_workspace_bytes",
+    "dsa_plan_pages",
+    "dsa_append_kv",
 )
 
 # Bytes per token of the FP8 KV cache (DSA_FP8_ROW_BYTES in include/dsa_b200.h).
@@ -74,6 +78,43 @@ class IndexerArgs(ctypes.Structure):
         ("batch", ctypes.c_int64), ("queries", ctypes.c_int64), ("heads", ctypes.c_int64),
         ("length", ctypes.c_int64), ("topk", ctypes.c_int64),
         ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64), ("status", ctypes.c_void_p),
+    ]
+
+
+DTYPE_BF16, DTYPE_FP16, DTYPE_FP32 = 0, 1, 2
+ROPE_LAYOUTS = {"interleaved": 0, "half": 1}
+
+
+class RotaryArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", ctypes.c_void_p), ("y", ctypes.c_void_p), ("positions", ctypes.c_void_p), ("inv_freq", ctypes.c_void_p),
+        ("batch", ctypes.c_int64), ("queries", ctypes.c_int64), ("heads", ctypes.c_int64), ("dim", ctypes.c_int64),
+        # x_stride[3], y_stride[3], position_stride[2]
+        *[(f"x_stride_{k}", ctypes.c_int64) for k in range(3)], *[(f"y_stride_{k}", ctypes.c_int64) for k in range(3)],
+        *[(f"position_stride_{k}", ctypes.c_int64) for k in range(2)],
+        ("rotary_dim", ctypes.c_int32), ("start", ctypes.c_int32), ("dtype", ctypes.c_int32),
+        ("positions64", ctypes.c_int32), ("layout", ctypes.c_int32), ("inverse", ctypes.c_int32),
+        ("attention_factor", ctypes.c_float),
+    ]
+
+
+class PlanPagesArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in (
+        "block_table", "cached_lens", "new_lens", "free_blocks", "free_count", "reset", "table_out", "seq_lens",
+        "positions", "lengths", "slots", "free_blocks_out", "free_count_out", "missing")] + [
+        ("batch", ctypes.c_int64), ("queries", ctypes.c_int64), ("max_blocks", ctypes.c_int64),
+        ("num_blocks", ctypes.c_int64), ("block_size", ctypes.c_int64),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64),
+    ]
+
+
+class AppendKvArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in (
+        "kv", "k_rope", "slots", "positions", "inv_freq", "kv_cache", "k_rope_cache", "cache")] + [
+        ("batch", ctypes.c_int64), ("queries", ctypes.c_int64), ("rows", ctypes.c_int64),
+        # kv_stride[2], k_rope_stride[2]
+        *[(f"kv_stride_{k}", ctypes.c_int64) for k in range(2)], *[(f"k_rope_stride_{k}", ctypes.c_int64) for k in range(2)],
+        ("layout", ctypes.c_int32), ("attention_factor", ctypes.c_float),
     ]
 
 
@@ -156,6 +197,14 @@ def _bind(lib):
     lib.dsa_indexer_workspace_bytes.argtypes = [ctypes.POINTER(IndexerArgs)]
     lib.dsa_indexer_topk.restype = ctypes.c_int
     lib.dsa_indexer_topk.argtypes = [ctypes.POINTER(IndexerArgs), ctypes.c_void_p]
+    lib.dsa_rotary.restype = ctypes.c_int
+    lib.dsa_rotary.argtypes = [ctypes.POINTER(RotaryArgs), ctypes.c_void_p]
+    lib.dsa_plan_pages_workspace_bytes.restype = ctypes.c_uint64
+    lib.dsa_plan_pages_workspace_bytes.argtypes = [ctypes.POINTER(PlanPagesArgs)]
+    lib.dsa_plan_pages.restype = ctypes.c_int
+    lib.dsa_plan_pages.argtypes = [ctypes.POINTER(PlanPagesArgs), ctypes.c_void_p]
+    lib.dsa_append_kv.restype = ctypes.c_int
+    lib.dsa_append_kv.argtypes = [ctypes.POINTER(AppendKvArgs), ctypes.c_void_p]
     lib.dsa_set_wait_test.restype = ctypes.c_int
     lib.dsa_set_wait_test.argtypes = [ctypes.c_uint64, ctypes.c_int]
     return lib

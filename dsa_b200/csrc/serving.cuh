@@ -1,0 +1,83 @@
+// Kernel parameters and launchers of the serving operators around the
+// forward: rotary positions (rotary.cu), page plans (pages.cu) and cache
+// appends (append.cu).
+#pragma once
+
+#include "dsa_common.cuh"
+
+namespace dsa {
+
+struct RotaryParams {
+  const void* x;
+  void* y;
+  const void* positions;  // int32 or int64 [batch, queries]
+  const double* inv_freq; // [rotary_dim / 2]
+  long long xs[3], ys[3]; // strides in elements: batch, query, head
+  long long ps[2];        // strides of positions
+  long long tokens;       // batch * queries
+  int queries, heads, dim, rotary_dim, start;
+  int pos64, half, in_place;
+  float factor;           // on cosines and sines
+  float sin_sign;         // -1 for the inverse rotation
+};
+cudaError_t launch_rotary(const RotaryParams& p, int dtype, cudaStream_t stream);
+
+struct PageParams {
+  const int32_t* table_in;    // [batch, max_blocks]
+  const int32_t* cached;      // [batch]
+  const int32_t* new_lens;    // [batch]
+  const int32_t* free_in;     // [num_blocks], a stack of free_count entries
+  const int32_t* free_count;  // [1]
+  const uint8_t* reset;       // [batch] or null
+  int32_t* table_out;
+  int32_t* seq_lens;          // [batch]
+  int32_t* positions;         // [batch, queries]
+  int32_t* lengths;           // [batch, queries]
+  int32_t* slots;             // [batch, queries]
+  int32_t* free_out;
+  int32_t* free_count_out;
+  int32_t* missing;           // [1]
+  int4* rows;                 // workspace: [batch] {start, new tokens, pages kept, first page taken}
+  int32_t* total;             // workspace: {stack height before the pages are taken, height without the returned pages}
+  int batch, queries, max_blocks, num_blocks, block_size;
+};
+cudaError_t launch_plan_pages(const PageParams& p, cudaStream_t stream);
+
+struct AppendParams {
+  const __nv_bfloat16* kv;      // rows of 512
+  const __nv_bfloat16* k_rope;  // rows of 64
+  const int32_t* slots;         // [batch, queries]
+  const int32_t* positions;     // [batch, queries] or null (k_rope is stored as given)
+  const double* inv_freq;       // [32] or null
+  __nv_bfloat16* kv_cache;      // [rows, 512] (BF16 cache)
+  __nv_bfloat16* rope_cache;    // [rows, 64] (BF16 cache)
+  uint8_t* cache;               // [rows, 656] (FP8 cache) or null
+  long long kvs[2], krs[2];     // strides in elements: batch, query
+  long long tokens, rows;
+  int queries, half;
+  float factor;
+};
+cudaError_t launch_append_kv(const AppendParams& p, cudaStream_t stream);
+
+#ifdef __CUDACC__
+// factor * (cos, sin) of the angle pos * freq. The angle is counted in turns
+// in FP64 and reduced there: an FP32 angle of position 10^6 would be off by
+// up to 2^-5 radians, the reduced one is within 2^-24 of a half turn for
+// every 32-bit position.
+__device__ __forceinline__ void rotary_cos_sin(long long pos, double freq, float factor, float sin_sign, float* c,
+                                               float* s) {
+  double t = (double)pos * freq * 0.15915494309189533577;  // 1 / (2 pi)
+  t -= rint(t);
+  float sn, cs;
+  sincospif((float)(t + t), &sn, &cs);
+  *c = cs * factor;
+  *s = sn * (factor * sin_sign);
+}
+// The turned pair, with the roundings spelled out: rotary and the cache
+// appends give the same bits.
+__device__ __forceinline__ float2 rotate_pair(float a, float b, float c, float s) {
+  return make_float2(__fmaf_rn(a, c, -__fmul_rn(b, s)), __fmaf_rn(b, c, __fmul_rn(a, s)));
+}
+#endif
+
+}  // namespace dsa

@@ -1,0 +1,169 @@
+"""Page plans and cache appends: what a serving step does before ``forward_paged``.
+
+``plan_pages`` builds, on the GPU, the block tables, token positions and cache
+slots of a step from the requests' lengths; ``append_kv`` / ``append_kv_fp8``
+write the new tokens' rows into the caches that ``forward_paged`` (or
+``forward``) and ``forward_fp8`` read. The reference has no cache management
+(README.md:19-20).
+
+A dense cache ``[B, L, 1, 512]`` is the page pool of ``B`` blocks of ``L``
+rows, so the slot of position ``p`` of row ``b`` is ``b * L + p``.
+"""
+from __future__ import annotations
+
+from collections import namedtuple
+
+import torch
+
+from . import _native, api
+from .rope import _check_rope
+
+PagePlan = namedtuple("PagePlan", "block_table seq_lens positions lengths slots free_blocks free_count missing")
+
+
+def plan_pages(block_table, cached_lens, new_lens, free_blocks, free_count, block_size, queries, *, reset=None,
+               inplace=False):
+    """Pages, positions and cache slots of ``new_lens[b]`` more tokens for every batch row.
+
+    ``block_table`` int32 ``[B, MB]`` and ``cached_lens`` int32 ``[B]`` describe
+    the cache so far; ``free_blocks`` int32 ``[NB]`` is a stack of
+    ``free_count`` (int32 ``[1]``) page numbers; ``queries`` is the padded
+    number of new tokens per row (``SQ`` of the step's tensors). ``reset``
+    (bool ``[B]``) gives rows to new requests: their pages go back on the stack
+    first and their cached length counts as 0 (with ``new_lens`` 0 the row is
+    only released). Rows take pages from the top of the stack, in order.
+
+    Returns a ``PagePlan`` of int32 tensors: the new ``block_table``,
+    ``seq_lens`` ``[B]``, ``positions``, ``lengths`` (positions + 1, the
+    indexer's key counts) and ``slots`` (cache rows, for ``append_kv``)
+    ``[B, SQ]``, the stack ``free_blocks`` and ``free_count``, and ``missing``
+    ``[1]``, the pages that the stack could not give: their table entries and
+    the slots of their tokens are -1, so that they are neither written nor
+    read. Padding has position and slot -1 and length 0. Lengths out of range
+    are clamped (to ``[0, SQ]`` new tokens and to the table's room).
+
+    New tensors are returned, unless ``inplace`` updates ``block_table``,
+    ``cached_lens`` (to ``seq_lens``), ``free_blocks`` and ``free_count``; the
+    call is asynchronous, allocates through torch and can be captured.
+    """
+    if block_table.dim() != 2 or type(block_size) is not int or type(queries) is not int or block_size <= 0 or queries <= 0:
+        raise ValueError("block_table must be 2-D, block_size and queries positive ints")
+    batch, max_blocks = block_table.shape
+    num_blocks = free_blocks.shape[0] if free_blocks.dim() == 1 else 0
+    rows = cached_lens.shape
+    if (not batch or not max_blocks or not num_blocks or rows != (batch,) or new_lens.shape != rows
+            or free_count.numel() != 1 or (reset is not None and reset.shape != rows)):
+        raise ValueError("need block_table[B,MB], cached_lens[B], new_lens[B], free_blocks[NB], free_count[1], reset[B]")
+    device, index = block_table.device, block_table.get_device()
+    if device.type != api.DEVICE_TYPE:
+        raise ValueError("all inputs must be contiguous and on the same CUDA device")
+    for t in (block_table, cached_lens, new_lens, free_blocks, free_count):
+        if t.get_device() != index or not t.is_contiguous():
+            raise ValueError("all inputs must be contiguous and on the same CUDA device")
+        if t.dtype != torch.int32:
+            raise ValueError("block_table, lengths and free pages must be int32 and reset bool")
+    if reset is not None:
+        if reset.get_device() != index or not reset.is_contiguous():
+            raise ValueError("all inputs must be contiguous and on the same CUDA device")
+        if reset.dtype != torch.bool:
+            raise ValueError("block_table, lengths and free pages must be int32 and reset bool")
+    if max(max_blocks, num_blocks) * block_size > 0x7fffffff or batch * max(queries, max_blocks) > 0x7fffffff:
+        raise ValueError("a table, the page pool or the step holds more than 2^31 - 1 entries")
+    # few allocations and views: they cost more host time than the kernels take
+    positions, lengths, slots = torch.empty((3, batch, queries), dtype=torch.int32, device=device).unbind(0)
+    work_words = 4 * batch + 4
+    small = torch.empty(work_words + 2 + batch, dtype=torch.int32, device=device)
+    _, missing, count, lens = small.split_with_sizes((work_words, 1, 1, batch))
+    if inplace:
+        table, lens, stack, count = block_table, cached_lens, free_blocks, free_count
+    else:
+        table, stack = torch.empty_like(block_table), torch.empty_like(free_blocks)
+    api.enqueue("dsa_plan_pages", _native.PlanPagesArgs(
+        block_table.data_ptr(), cached_lens.data_ptr(), new_lens.data_ptr(), free_blocks.data_ptr(),
+        free_count.data_ptr(), None if reset is None else reset.data_ptr(), table.data_ptr(), lens.data_ptr(),
+        positions.data_ptr(), lengths.data_ptr(), slots.data_ptr(), stack.data_ptr(), count.data_ptr(),
+        missing.data_ptr(), batch, queries, max_blocks, num_blocks, block_size, small.data_ptr(), 4 * work_words), index)
+    return PagePlan(table, lens, positions, lengths, slots, stack, count, missing)
+
+
+def _append(kv, k_rope, slots, latent, rope, fp8, positions, inv_freq, layout, attention_factor):
+    """Checks and launch; the caches are ``latent`` and ``rope``, or ``fp8``."""
+    shape, index = kv.shape, kv.get_device()
+    if len(shape) != 4 or shape[2:] != (1, 512) or 0 in shape or k_rope.shape != (*shape[:3], 64):
+        raise ValueError("need kv[B,S,1,512] and k_rope[B,S,1,64]")
+    lead = shape[:2]
+    if slots.shape != lead or slots.dtype != torch.int32:
+        raise ValueError("slots must be int32 [B,S]")
+    if kv.dtype != torch.bfloat16 or k_rope.dtype != torch.bfloat16:
+        raise ValueError("kv and k_rope must be bfloat16")
+    (kv0, kv1, _, kv3), (kr0, kr1, _, kr3) = kv.stride(), k_rope.stride()
+    if kv3 != 1 or kr3 != 1:
+        raise ValueError("the last dimension of kv and k_rope must be contiguous")
+    if kv.device.type != api.DEVICE_TYPE or k_rope.get_device() != index or slots.get_device() != index:
+        raise ValueError("all inputs must be on the same CUDA device")
+    if not slots.is_contiguous():
+        raise ValueError("slots and the cache must be contiguous")
+    for cache in (latent, rope) if fp8 is None else (fp8,):
+        if cache.get_device() != index:
+            raise ValueError("all inputs must be on the same CUDA device")
+        if not cache.is_contiguous():
+            raise ValueError("slots and the cache must be contiguous")
+        rows = cache.shape[0] * cache.shape[1]
+    if (positions is None) != (inv_freq is None):
+        raise ValueError("positions and inv_freq go together")
+    if inv_freq is not None:
+        number = _check_rope(positions, inv_freq, layout, attention_factor, lead, index)
+        if positions.dtype != torch.int32 or not positions.is_contiguous() or inv_freq.shape[0] != 32:
+            raise ValueError("positions must be contiguous int32 [B,S] and inv_freq have 32 entries")
+    elif layout in _native.ROPE_LAYOUTS:
+        number, attention_factor = 0, 1.0
+    else:
+        raise ValueError("layout must be 'interleaved' or 'half'")
+    batch, queries = lead
+    if rows > 0x7fffffff or batch * queries > 0x7fffffff:
+        raise ValueError("the cache or the step holds more than 2^31 - 1 rows")
+    api.enqueue("dsa_append_kv", _native.AppendKvArgs(
+        kv.data_ptr(), k_rope.data_ptr(), slots.data_ptr(), None if positions is None else positions.data_ptr(),
+        None if inv_freq is None else inv_freq.data_ptr(), None if latent is None else latent.data_ptr(),
+        None if rope is None else rope.data_ptr(), None if fp8 is None else fp8.data_ptr(), batch, queries, rows,
+        kv0, kv1, kr0, kr1, number, attention_factor), index)
+
+
+def append_kv(kv, k_rope, slots, kv_cache, k_rope_cache, *, positions=None, inv_freq=None, layout="interleaved",
+              attention_factor=1.0):
+    """Write the new tokens' rows into a BF16 cache, in place.
+
+    ``kv`` ``[B, S, 1, 512]`` and ``k_rope`` ``[B, S, 1, 64]`` BF16 (any
+    strides with the last dimension contiguous: slices of the projection's
+    output will do) go to the rows ``slots`` (int32 ``[B, S]``) of
+    ``kv_cache`` ``[NB, BS, 1, 512]`` / ``k_rope_cache`` ``[NB, BS, 1, 64]``,
+    flattened over the first two dimensions. A slot outside the cache writes
+    nothing (padding is -1); the other rows keep what they hold. Slots of one
+    call must be distinct (those of a plan are). With ``positions`` (int32
+    ``[B, S]``) and ``inv_freq`` (FP64 ``[32]``) ``k_rope`` is turned first, as
+    by ``rotary``; without them it is stored as given.
+    """
+    if (kv_cache.dim() != 4 or k_rope_cache.dim() != 4 or kv_cache.shape[2:] != (1, 512) or 0 in kv_cache.shape
+            or k_rope_cache.shape != (*kv_cache.shape[:3], 64)):
+        raise ValueError("need kv_cache[NB,BS,1,512] and k_rope_cache[NB,BS,1,64]")
+    if kv_cache.dtype != torch.bfloat16 or k_rope_cache.dtype != torch.bfloat16:
+        raise ValueError("the caches must be bfloat16")
+    _append(kv, k_rope, slots, kv_cache, k_rope_cache, None, positions, inv_freq, layout, attention_factor)
+
+
+def append_kv_fp8(kv, k_rope, slots, cache, *, positions=None, inv_freq=None, layout="interleaved",
+                  attention_factor=1.0):
+    """``append_kv`` into the FP8 rows that ``forward_fp8`` reads.
+
+    ``cache`` is uint8 ``[NB, BS, 1, 656]`` (``[B, L, 1, 656]`` for
+    ``forward_fp8``). A row holds what ``quantize_kv_fp8`` makes of the same
+    token on the host, bit for bit, with ``k_rope`` turned first when
+    ``positions`` and ``inv_freq`` are given. (On the GPU that function's
+    ``amax / 448`` is torch's product with the rounded 1 / 448, so its scales
+    may be one FP32 step away.)
+    """
+    if cache.dim() != 4 or cache.shape[2:] != (1, _native.FP8_ROW_BYTES) or 0 in cache.shape:
+        raise ValueError("need cache[NB,BS,1,656]")
+    if cache.dtype != torch.uint8:
+        raise ValueError("the FP8 cache must be uint8")
+    _append(kv, k_rope, slots, None, None, cache, positions, inv_freq, layout, attention_factor)

@@ -229,6 +229,106 @@ DSA_B200_API uint64_t dsa_indexer_workspace_bytes(const dsa_indexer_args_t* args
 /* Indexer scores then top-k, two kernels on `stream`. Returns a dsa_status_t. */
 DSA_B200_API int dsa_indexer_topk(const dsa_indexer_args_t* args, void* stream);
 
+/* Rotary positions (no counterpart in the reference, which takes q_rope and
+ * k_rope already turned): y = x with rotary_dim of its dim elements, from
+ * `start` on, turned by t = positions[b][s] * inv_freq[i],
+ *   y_a = f (x_a cos t - x_b sin t),  y_b = f (x_b cos t + x_a sin t)
+ * over the pairs (2i, 2i + 1) (interleaved) or (i, i + rotary_dim / 2) (half),
+ * f = attention_factor, and -t when `inverse` is set (which is also the
+ * gradient of the forward map). The other elements are copied. The angle is
+ * reduced in FP64, cosines and products are FP32, one rounding to the type. y
+ * may be x (same pointer and strides) and overlaps it in no other way. */
+typedef enum dsa_dtype { DSA_BF16 = 0, DSA_FP16 = 1, DSA_FP32 = 2 } dsa_dtype_t;
+typedef enum dsa_rope_layout { DSA_ROPE_INTERLEAVED = 0, DSA_ROPE_HALF = 1 } dsa_rope_layout_t;
+typedef struct dsa_rotary_args {
+  const void* x;             /* [batch, queries, heads, dim], last dim contiguous */
+  void* y;                   /* same shape and type */
+  const void* positions;     /* [batch, queries] INT32, or INT64 with positions64 */
+  const double* inv_freq;    /* FP64 [rotary_dim / 2], radians per position */
+  int64_t batch, queries, heads, dim;
+  int64_t x_stride[3], y_stride[3];  /* batch, query, head, in elements */
+  int64_t position_stride[2];        /* batch, query */
+  int32_t rotary_dim, start;
+  int32_t dtype;             /* dsa_dtype_t */
+  int32_t positions64;
+  int32_t layout;            /* dsa_rope_layout_t */
+  int32_t inverse;
+  float attention_factor;
+} dsa_rotary_args_t;
+
+/* One kernel on `stream`. Returns a dsa_status_t. */
+DSA_B200_API int dsa_rotary(const dsa_rotary_args_t* args, void* stream);
+
+/* Page plan of one serving step over a paged cache (no counterpart in the
+ * reference). Row b has cached_lens[b] tokens (0 when reset[b] is set: the row
+ * is given to a new request, and its pages go back on the stack of free pages
+ * first) and gets n = new_lens[b] more, at most `queries` and the table's
+ * room. It keeps its pages and takes those that its new tokens start, rows in
+ * order, from the top of the stack free_blocks[0 .. free_count). Out:
+ *   table_out      the table with the pages taken (-1: none was left; a reset
+ *                  row's entries past its pages are -1, others are copied)
+ *   seq_lens       cached + new tokens
+ *   positions      [batch, queries] position of each new token, -1 for padding
+ *   lengths        positions + 1 (the key counts of dsa_indexer_topk)
+ *   slots          table_out[pos / block_size] * block_size + pos % block_size,
+ *                  the row of dsa_append_kv; -1 for padding or without a page
+ *   free_blocks_out, free_count_out   the stack afterwards
+ *   missing        pages that were wanted and not there
+ * In place: table_out, seq_lens, free_blocks_out and free_count_out may be
+ * block_table, cached_lens, free_blocks and free_count. Counts and lengths out
+ * of range are clamped; table entries outside [0, num_blocks) name no page. */
+typedef struct dsa_plan_pages_args {
+  const int32_t* block_table;  /* [batch, max_blocks] */
+  const int32_t* cached_lens;  /* [batch] */
+  const int32_t* new_lens;     /* [batch] */
+  const int32_t* free_blocks;  /* [num_blocks] */
+  const int32_t* free_count;   /* [1] */
+  const uint8_t* reset;        /* [batch] or NULL */
+  int32_t* table_out;
+  int32_t* seq_lens;
+  int32_t* positions;
+  int32_t* lengths;
+  int32_t* slots;
+  int32_t* free_blocks_out;
+  int32_t* free_count_out;
+  int32_t* missing;            /* [1] */
+  int64_t batch, queries, max_blocks, num_blocks, block_size;
+  void* workspace;
+  uint64_t workspace_bytes;
+} dsa_plan_pages_args_t;
+
+/* Workspace bytes of dsa_plan_pages; 0 for invalid sizes. */
+DSA_B200_API uint64_t dsa_plan_pages_workspace_bytes(const dsa_plan_pages_args_t* args);
+
+/* Two kernels on `stream`. Returns a dsa_status_t. */
+DSA_B200_API int dsa_plan_pages(const dsa_plan_pages_args_t* args, void* stream);
+
+/* Cache append (no counterpart in the reference): row slots[b][s] of the
+ * cache gets token (b, s)'s latent and rope part, the rope part turned as by
+ * dsa_rotary when inv_freq is given. With `cache` the row is the FP8 row of
+ * dsa_sparse_mla_fwd_fp8 (scale k = max |kv| over its 128 dims / 448, 1 for a
+ * block of zeros), else kv_cache / k_rope_cache are the BF16 rows of
+ * dsa_sparse_mla_fwd(_paged). A slot outside [0, rows) writes nothing. Slots
+ * of one call are distinct; of two tokens with one slot either may win, or
+ * parts of both. */
+typedef struct dsa_append_kv_args {
+  const void* kv;            /* BF16 [batch, queries, 512], last dim contiguous */
+  const void* k_rope;        /* BF16 [batch, queries, 64], last dim contiguous */
+  const int32_t* slots;      /* [batch, queries] */
+  const int32_t* positions;  /* [batch, queries], or NULL without inv_freq */
+  const double* inv_freq;    /* FP64 [32], or NULL: k_rope is stored as given */
+  void* kv_cache;            /* BF16 [rows, 512], or NULL with `cache` */
+  void* k_rope_cache;        /* BF16 [rows, 64], or NULL with `cache` */
+  void* cache;               /* uint8 [rows, 656], or NULL */
+  int64_t batch, queries, rows;
+  int64_t kv_stride[2], k_rope_stride[2];  /* batch, query, in elements */
+  int32_t layout;            /* dsa_rope_layout_t */
+  float attention_factor;
+} dsa_append_kv_args_t;
+
+/* One kernel on `stream`. Returns a dsa_status_t. */
+DSA_B200_API int dsa_append_kv(const dsa_append_kv_args_t* args, void* stream);
+
 /* Number of kernels the last successful dsa_sparse_mla_fwd on this host
  * thread enqueued (1 or 2), for launch accounting. Calls of
  * dsa_sparse_mla_fwd_noalloc do not update it. */

@@ -1,0 +1,63 @@
+"""Page plans and cache appends on the CPU: the argument rules; GPU parity is in test_gpu_paging.py."""
+import ctypes
+
+import pytest
+import torch
+
+import dsa_b200
+from dsa_b200 import _native, api
+
+
+def t(*shape, dtype=torch.int32):
+    return torch.empty(shape, dtype=dtype, device="meta")
+
+
+def test_plan_refusals(monkeypatch):
+    monkeypatch.setattr(api, "DEVICE_TYPE", "meta")
+    good = dict(block_table=t(4, 8), cached_lens=t(4), new_lens=t(4), free_blocks=t(32), free_count=t(1), block_size=16,
+                queries=5)
+    for change, why in [
+        (dict(block_table=t(4)), "2-D"), (dict(block_size=0), "positive"), (dict(queries=0), "positive"),
+        (dict(queries=2.0), "positive"), (dict(cached_lens=t(3)), "need block_table"),
+        (dict(new_lens=t(4, 1)), "need block_table"), (dict(free_blocks=t(4, 8)), "need block_table"),
+        (dict(free_blocks=t(0)), "need block_table"), (dict(free_count=t(2)), "need block_table"),
+        (dict(reset=t(3, dtype=torch.bool)), "need block_table"), (dict(reset=t(4)), "reset bool"),
+        (dict(block_table=t(4, 8, dtype=torch.int64)), "int32"), (dict(block_table=t(8, 4).t()), "contiguous"),
+        (dict(block_size=1 << 30), "2\\^31"), (dict(queries=1 << 30), "2\\^31"),
+    ]:
+        with pytest.raises(ValueError, match=why):
+            dsa_b200.plan_pages(**{**good, **change})
+
+
+def test_plan_workspace_bytes():
+    lib, a = _native.load(), _native.PlanPagesArgs()
+    a.batch, a.queries, a.max_blocks, a.num_blocks, a.block_size = 5, 3, 8, 100, 64
+    assert lib.dsa_plan_pages_workspace_bytes(ctypes.byref(a)) >= 5 * 16
+    a.block_size = 1 << 30
+    assert lib.dsa_plan_pages_workspace_bytes(ctypes.byref(a)) == 0
+
+
+def test_append_refusals(monkeypatch):
+    monkeypatch.setattr(api, "DEVICE_TYPE", "meta")
+    bf, f64 = torch.bfloat16, torch.float64
+    kv, kr, slots = t(2, 3, 1, 512, dtype=bf), t(2, 3, 1, 64, dtype=bf), t(2, 3)
+    pool, rope = t(9, 16, 1, 512, dtype=bf), t(9, 16, 1, 64, dtype=bf)
+    for args, kw, why in [
+        ((t(2, 3, 512, dtype=bf), kr, slots, pool, rope), {}, "need kv"),
+        ((kv, t(2, 3, 1, 32, dtype=bf), slots, pool, rope), {}, "need kv"),
+        ((kv, kr, t(2, 4), pool, rope), {}, "slots"),
+        ((kv, kr, t(2, 3, dtype=torch.int64), pool, rope), {}, "slots"),
+        ((kv.float(), kr, slots, pool, rope), {}, "bfloat16"),
+        ((kv, kr, slots, pool, t(9, 15, 1, 64, dtype=bf)), {}, "need kv_cache"),
+        ((kv, kr, slots, pool.float(), rope), {}, "caches must be"),
+        ((kv, kr, slots, pool, rope), dict(positions=t(2, 3)), "go together"),
+        ((kv, kr, slots, pool, rope), dict(positions=t(2, 3), inv_freq=t(16, dtype=f64)), "32 entries"),
+        ((kv, kr, slots, pool, rope), dict(positions=t(2, 3, dtype=torch.int64), inv_freq=t(32, dtype=f64)), "int32"),
+        ((kv, kr, slots, pool, rope), dict(layout="other"), "layout"),
+        ((kv, kr, slots, t(16, 9, 1, 512, dtype=bf).transpose(0, 1), rope), {}, "contiguous"),
+    ]:
+        with pytest.raises(ValueError, match=why):
+            dsa_b200.append_kv(*args, **kw)
+    for cache, why in [(t(9, 16, 1, 655, dtype=torch.uint8), "need cache"), (t(9, 16, 1, 656, dtype=torch.int8), "uint8")]:
+        with pytest.raises(ValueError, match=why):
+            dsa_b200.append_kv_fp8(kv, kr, slots, cache)

@@ -1,0 +1,64 @@
+"""Rotary positions on the CPU: the frequencies and the argument rules; GPU parity is in test_gpu_rope.py."""
+import math
+
+import pytest
+import torch
+
+import dsa_b200
+from dsa_b200 import api
+
+
+def test_frequencies():
+    f = dsa_b200.rotary_frequencies(64, 10000.0)
+    assert f.dtype == torch.float64 and f.shape == (32,) and f[0] == 1.0
+    assert math.isclose(f[31].item(), 10000.0 ** (-62 / 64), rel_tol=1e-14)
+    assert torch.equal(dsa_b200.rotary_frequencies(64, scaling="linear", factor=8.0), f / 8.0)
+    ntk = dsa_b200.rotary_frequencies(64, scaling="ntk", factor=8.0)
+    # the fastest pair is kept, the slowest divided by the factor: theta'^(-62/64) = theta^(-62/64) / 8
+    assert ntk[0] == 1.0 and math.isclose(ntk[31].item(), f[31].item() / 8.0, rel_tol=1e-12)
+    yarn = dsa_b200.rotary_frequencies(64, scaling="yarn", factor=40.0, original_length=4096)
+    turns = 4096 * f / (2 * math.pi)
+    assert torch.equal(yarn[turns > 40], f[turns > 40]) and torch.equal(yarn[turns < 0.7], f[turns < 0.7] / 40.0)
+    assert bool(((yarn <= f) & (yarn >= f / 40.0)).all()) and bool((yarn[1:] < yarn[:-1]).all())
+
+
+@pytest.mark.parametrize("kw", [dict(rotary_dim=7), dict(rotary_dim=0), dict(rotary_dim=64, theta=1.0),
+                                dict(rotary_dim=64, factor=0.5), dict(rotary_dim=64, scaling="other"),
+                                dict(rotary_dim=64, scaling="yarn", factor=4.0),
+                                dict(rotary_dim=2, scaling="ntk", factor=4.0)])
+def test_frequency_refusals(kw):
+    with pytest.raises(ValueError):
+        dsa_b200.rotary_frequencies(**kw)
+
+
+def test_rotary_refusals(monkeypatch):
+    monkeypatch.setattr(api, "DEVICE_TYPE", "meta")
+
+    def t(*shape, dtype=torch.bfloat16):
+        return torch.empty(shape, dtype=dtype, device="meta")
+
+    x, pos, freq = t(2, 3, 4, 64), t(2, 3, dtype=torch.int32), t(32, dtype=torch.float64)
+    for args, kw, why in [
+        ((t(2, 3), pos, freq), {}, "x must be"),
+        ((t(2, 0, 4, 64), t(2, 0, dtype=torch.int32), freq), {}, "x must be"),
+        ((t(2, 3, 4, 64, dtype=torch.float64), pos, freq), {}, "bfloat16, float16 or float32"),
+        ((x, t(2, 4, dtype=torch.int32), freq), {}, "positions"),
+        ((x, pos.float(), freq), {}, "positions"),
+        ((x, pos, freq.float()), {}, "float64"),
+        ((x, pos, t(33, dtype=torch.float64)), {}, "start"),
+        ((x, pos, t(16, dtype=torch.float64)), dict(start=33), "start"),
+        ((x, pos, t(16, dtype=torch.float64)), dict(start=-1), "start"),
+        ((x, pos, t(0, dtype=torch.float64)), {}, "start"),
+        ((x, pos, freq), dict(layout="other"), "layout"),
+        ((x, pos, freq), dict(attention_factor=float("nan")), "attention_factor"),
+        ((t(2, 3, 64, 4).transpose(2, 3), pos, freq), {}, "last dimension"),
+        ((x, pos, freq), dict(out=t(2, 3, 4, 63)), "out must"),
+        ((x, pos, freq), dict(out=t(2, 3, 1, 64).expand(2, 3, 4, 64)), "out must"),
+        ((x, pos, t(32, dtype=torch.float64).requires_grad_()), {}, "gradient"),
+    ]:
+        with pytest.raises(ValueError, match=why):
+            dsa_b200.rotary(*args, **kw)
+    with pytest.raises(ValueError, match="CUDA device"):
+        dsa_b200.rotary(torch.empty(2, 3, 4, 64, dtype=torch.bfloat16), pos, freq)
+    with pytest.raises(ValueError, match="autograd"):
+        dsa_b200.rotary(t(2, 3, 4, 64).requires_grad_(), pos, t(32, dtype=torch.float64), out=t(2, 3, 4, 64))
