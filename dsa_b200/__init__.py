@@ -9,10 +9,11 @@ from .fp8_cache import quantize_kv_fp8
 from .indexer import indexer_topk
 from .paging import PagePlan, append_kv, append_kv_fp8, plan_pages
 from .rope import rotary, rotary_frequencies
+from .shared_prefix import forward_shared_prefix
 from .config import CASE_SHAPES, SELECTED, Tuning
 from .sparse_flash_attention import npu_sparse_flash_attention, sparse_flash_attention
 
 __all__ = ["forward", "forward_paged", "forward_fp8", "quantize_kv_fp8", "indexer_topk", "rotary", "rotary_frequencies",
-           "plan_pages", "PagePlan", "append_kv", "append_kv_fp8", "ForwardPlan", "Tuning", "CASE_SHAPES", "SELECTED", "device_status",
+           "forward_shared_prefix", "plan_pages", "PagePlan", "append_kv", "append_kv_fp8", "ForwardPlan", "Tuning", "CASE_SHAPES", "SELECTED", "device_status",
            "check_device_status", "clear_device_status", "sparse_flash_attention",
            "npu_sparse_flash_attention"]

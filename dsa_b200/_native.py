@@ -51,6 +51,8 @@ EXPORTS = (
     "dsa_plan_pages_workspace_bytes",
     "dsa_plan_pages",
     "dsa_append_kv",
+    "dsa_fwd_prefix_workspace_bytes",
+    "dsa_sparse_mla_fwd_prefix",
 )
 
 # Bytes per token of the FP8 KV cache (DSA_FP8_ROW_BYTES in include/dsa_b200.h).
@@ -69,6 +71,11 @@ class Launch(ctypes.Structure):
 class PagedKv(ctypes.Structure):
     _fields_ = [("block_table", ctypes.c_void_p), ("seq_lens", ctypes.c_void_p),
                 ("max_blocks", ctypes.c_int64), ("block_size", ctypes.c_int64), ("num_blocks", ctypes.c_int64)]
+
+
+class PrefixKv(ctypes.Structure):
+    _fields_ = [("kv", ctypes.c_void_p), ("k_rope", ctypes.c_void_p), ("length", ctypes.c_void_p),
+                ("rows", ctypes.c_int64)]
 
 
 class IndexerArgs(ctypes.Structure):
@@ -197,6 +204,10 @@ def _bind(lib):
     lib.dsa_indexer_workspace_bytes.argtypes = [ctypes.POINTER(IndexerArgs)]
     lib.dsa_indexer_topk.restype = ctypes.c_int
     lib.dsa_indexer_topk.argtypes = [ctypes.POINTER(IndexerArgs), ctypes.c_void_p]
+    lib.dsa_fwd_prefix_workspace_bytes.restype = ctypes.c_uint64
+    lib.dsa_fwd_prefix_workspace_bytes.argtypes = [ctypes.POINTER(FwdArgs), ctypes.POINTER(PrefixKv)]
+    lib.dsa_sparse_mla_fwd_prefix.restype = ctypes.c_int
+    lib.dsa_sparse_mla_fwd_prefix.argtypes = [ctypes.POINTER(FwdArgs), ctypes.POINTER(PrefixKv), ctypes.c_void_p]
     lib.dsa_rotary.restype = ctypes.c_int
     lib.dsa_rotary.argtypes = [ctypes.POINTER(RotaryArgs), ctypes.c_void_p]
     lib.dsa_plan_pages_workspace_bytes.restype = ctypes.c_uint64

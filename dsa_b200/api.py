@@ -176,16 +176,17 @@ def _launch_native(args, stream_handle):
     return lib.dsa_last_launch_count()
 
 
-def enqueue(name, args, index):
-    """Call the C entry ``name(args, stream)`` on CUDA device ``index`` and its current stream; raise for its status."""
+def enqueue(name, args, index, *more):
+    """Call the C entry ``name(args, *more, stream)`` on CUDA device ``index`` and its current stream; raise for its
+    status."""
     call = getattr(_native.load(), name)
     if DEVICE_TYPE != "cuda":
-        code = call(args, 0)
+        code = call(args, *more, 0)
     elif index == torch.cuda.current_device():
-        code = call(args, torch._C._cuda_getCurrentRawStream(index))
+        code = call(args, *more, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):
-            code = call(args, torch._C._cuda_getCurrentRawStream(index))
+            code = call(args, *more, torch._C._cuda_getCurrentRawStream(index))
     if code != _native.STATUS_OK:
         _native.raise_for_status(code, name)
 

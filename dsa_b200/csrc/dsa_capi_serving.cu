@@ -1,13 +1,14 @@
 // extern "C" boundary of the serving operators (declared in
 // include/dsa_b200.h): what the C ABI can see is checked here (null pointers,
 // sizes, alignment), shapes and dtypes in the Python mirrors
-// (dsa_b200/rope.py, dsa_b200/paging.py).
+// (dsa_b200/rope.py, dsa_b200/paging.py, dsa_b200/shared_prefix.py).
 #include <cuda_runtime.h>
 
 #include <cmath>
 #include <cstring>
 
 #include "../../include/dsa_b200.h"
+#include "prefix.cuh"
 #include "serving.cuh"
 
 namespace {
@@ -24,6 +25,79 @@ int launch_status(cudaError_t err) { return err == cudaSuccess ? DSA_STATUS_OK :
 bool plan_ok(const dsa_plan_pages_args_t* a) {
   return a != nullptr && product_ok(a->batch, a->queries) && product_ok(a->batch, a->max_blocks) &&
          product_ok(a->max_blocks, a->block_size) && product_ok(a->num_blocks, a->block_size);
+}
+
+constexpr uint64_t kAlign = 256;
+uint64_t align_up(uint64_t x) { return (x + kAlign - 1) / kAlign * kAlign; }
+
+// Launches of one shared-prefix call and its workspace.
+struct PrefixPlan {
+  int64_t tokens, rows, row_tiles;
+  int split, own_split;  // own_split 0: no own keys
+  bool direct;           // the prefix kernel writes the output
+  uint64_t num, max, sum, own_num, own_max, own_sum, total;
+};
+
+// Key splits of the prefix: a cluster's time is its tiles plus a start of
+// about six (launch, TMEM, first loads), in waves of the resident clusters;
+// split partials cost a write and a read of 2 KB a row, about 5 TB/s (a tile
+// of 64 keys takes ~0.6 us).
+int prefix_split(int64_t row_tiles, int64_t keys, int clusters) {
+  const int64_t tiles = (keys + 63) / 64;
+  double best = 0;
+  int split = 1;
+  for (int s = 1; s <= 128 && s <= tiles; ++s) {
+    const int64_t waves = (row_tiles * s + clusters - 1) / clusters;
+    const double us = 0.6 * (double)waves * (double)((tiles + s - 1) / s + 6) +
+                      (s > 1 ? (double)row_tiles * s * 128 * 4096 / 5e6 : 0.0);
+    if (s == 1 || us < best) {
+      best = us;
+      split = s;
+    }
+  }
+  return split;
+}
+
+bool plan_prefix(const dsa_fwd_args_t* a, const dsa_prefix_kv_t* px, PrefixPlan* plan) {
+  if (a == nullptr || px == nullptr || a->launch.family != DSA_FAMILY_AUTO) return false;
+  if (!product_ok(a->batch, a->queries) || a->heads <= 0 || a->heads > 65536 || a->heads % 16 != 0) return false;
+  if (px->rows <= 0 || px->rows > (1LL << 30)) return false;
+  const bool own = a->topk > 0;
+  if (a->topk < 0 || a->topk > kMaxInt || (own && (!product_ok(a->batch, a->length)))) return false;
+  plan->tokens = a->batch * a->queries;
+  if (!product_ok(plan->tokens, a->heads, 1LL << 37)) return false;
+  plan->rows = plan->tokens * a->heads;
+  plan->row_tiles = (plan->rows + 127) / 128;
+  int clusters = dsa::prefix_max_clusters();
+  if (clusters <= 0) clusters = 74;
+  plan->split = prefix_split(plan->row_tiles, px->rows, clusters);
+  if (plan->row_tiles * plan->split > kMaxInt / 2) return false;
+  plan->own_split = 0;
+  if (own) {
+    // own keys: one wave of the pair (H = 128) or stream family's CTAs, two
+    // tiles of 32 keys at least per split
+    const int64_t tiles = (a->topk + 31) / 32;
+    int64_t ctas = a->heads == 128 ? dsa::pair_max_ctas() / 2 : dsa::stream_max_ctas();
+    if (ctas <= 0) ctas = a->heads == 128 ? 74 : 296;
+    int64_t s = ctas / (a->heads == 128 ? plan->tokens : plan->tokens * (a->heads / 16));
+    if (s > tiles / 2) s = tiles / 2;
+    if (s > 16) s = 16;
+    plan->own_split = (int)(s < 1 ? 1 : s);
+  }
+  plan->direct = !own && plan->split == 1;
+  plan->num = plan->max = plan->sum = plan->own_num = plan->own_max = plan->own_sum = plan->total = 0;
+  if (plan->direct) return true;
+  const uint64_t parts = (uint64_t)plan->row_tiles * (uint64_t)plan->split * 128u;
+  plan->max = align_up(parts * dsa::kDimLatent * 4u);
+  plan->sum = plan->max + align_up(parts * 4u);
+  plan->total = plan->own_num = plan->sum + align_up(parts * 4u);
+  if (own) {
+    const uint64_t mine = (uint64_t)plan->rows * (uint64_t)plan->own_split;
+    plan->own_max = plan->own_num + align_up(mine * dsa::kDimLatent * 4u);
+    plan->own_sum = plan->own_max + align_up(mine * 4u);
+    plan->total = plan->own_sum + align_up(mine * 4u);
+  }
+  return true;
 }
 
 }  // namespace
@@ -139,6 +213,88 @@ int dsa_append_kv(const dsa_append_kv_args_t* a, void* stream) {
   p.half = a->layout == DSA_ROPE_HALF;
   p.factor = a->attention_factor;
   return launch_status(dsa::launch_append_kv(p, static_cast<cudaStream_t>(stream)));
+}
+
+uint64_t dsa_fwd_prefix_workspace_bytes(const dsa_fwd_args_t* a, const dsa_prefix_kv_t* px) {
+  PrefixPlan plan;
+  return plan_prefix(a, px, &plan) ? plan.total : 0;
+}
+
+int dsa_sparse_mla_fwd_prefix(const dsa_fwd_args_t* a, const dsa_prefix_kv_t* px, void* stream) {
+  PrefixPlan plan;
+  if (!plan_prefix(a, px, &plan)) return DSA_STATUS_BAD_ARGUMENT;
+  const bool own = a->topk > 0;
+  if (!a->q || !a->q_rope || !a->output || !a->softmax_max || !a->softmax_sum || !px->kv || !px->k_rope)
+    return DSA_STATUS_BAD_ARGUMENT;
+  if (own != (a->kv != nullptr) || own != (a->k_rope != nullptr) || own != (a->indices != nullptr))
+    return DSA_STATUS_BAD_ARGUMENT;
+  if (!aligned(a->q, 16) || !aligned(a->q_rope, 16) || !aligned(a->output, 16) || !aligned(px->kv, 16) ||
+      !aligned(px->k_rope, 16) || !aligned(a->kv, 16) || !aligned(a->k_rope, 16) || !aligned(px->length, 4))
+    return DSA_STATUS_BAD_ARGUMENT;
+  if (plan.total > 0 && (a->workspace == nullptr || a->workspace_bytes < plan.total || !aligned(a->workspace, kAlign)))
+    return DSA_STATUS_WORKSPACE_TOO_SMALL;
+  char* const ws = static_cast<char*>(a->workspace);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+
+  dsa::FwdParams f;
+  std::memset(&f, 0, sizeof(f));
+  if (!dsa::fill_scale(a->scale, f)) return DSA_STATUS_BAD_ARGUMENT;
+  dsa::PrefixParams p;
+  p.q = static_cast<const __nv_bfloat16*>(a->q);
+  p.q_rope = static_cast<const __nv_bfloat16*>(a->q_rope);
+  p.length = px->length;
+  p.out = static_cast<__nv_bfloat16*>(a->output);
+  p.out_max = a->softmax_max;
+  p.out_sum = a->softmax_sum;
+  p.part_num = plan.direct ? nullptr : reinterpret_cast<float*>(ws + plan.num);
+  p.part_max = reinterpret_cast<float*>(ws + plan.max);
+  p.part_sum = reinterpret_cast<float*>(ws + plan.sum);
+  p.status = a->status;
+  p.rows = plan.rows;
+  p.keys = (int)px->rows;
+  p.split = plan.split;
+  p.scale_div = f.scale_div;
+  p.scale_log2 = f.scale_log2;
+  int st = launch_status(dsa::launch_fwd_prefix(p, px->kv, px->k_rope, s));
+  if (st != DSA_STATUS_OK || plan.direct) return st;
+
+  dsa::JoinParams j;
+  j.part_num = p.part_num;
+  j.part_max = p.part_max;
+  j.part_sum = p.part_sum;
+  j.own_num = reinterpret_cast<float*>(ws + plan.own_num);
+  j.own_max = reinterpret_cast<float*>(ws + plan.own_max);
+  j.own_sum = reinterpret_cast<float*>(ws + plan.own_sum);
+  j.out = p.out;
+  j.out_max = p.out_max;
+  j.out_sum = p.out_sum;
+  j.rows = plan.rows;
+  j.heads = (int)a->heads;
+  j.split = plan.split;
+  j.own_split = plan.own_split;
+  if (own) {
+    f.q = p.q;
+    f.q_rope = p.q_rope;
+    f.kv = static_cast<const __nv_bfloat16*>(a->kv);
+    f.k_rope = static_cast<const __nv_bfloat16*>(a->k_rope);
+    f.ids = a->indices;
+    f.part_num = reinterpret_cast<float*>(ws + plan.own_num);
+    f.part_max = reinterpret_cast<float*>(ws + plan.own_max);
+    f.part_sum = reinterpret_cast<float*>(ws + plan.own_sum);
+    f.status = a->status;
+    f.batch = (int)a->batch;
+    f.queries = (int)a->queries;
+    f.heads = (int)a->heads;
+    f.length = (int)a->length;
+    f.topk = (int)a->topk;
+    f.tokens = (int)plan.tokens;
+    f.split = plan.own_split;
+    f.keys_per_tile = 32;
+    f.heads_per_cta = a->heads == 128 ? 128 : 16;
+    st = launch_status(a->heads == 128 ? dsa::launch_fwd_pair(f, s) : dsa::launch_fwd_stream(f, s, false));
+    if (st != DSA_STATUS_OK) return st;
+  }
+  return launch_status(dsa::launch_prefix_join(j, s));
 }
 
 }  // extern "C"

@@ -755,7 +755,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) fwd_pair_kernel(const FwdParams
         if (e != 0) continue;
         const float f = (m_true == kNegFltMax) ? 1.f : ex2((m_w - m_true) * c);
         const size_t orow = (size_t)w.token * kPrHeads + row;
-        if (p.split == 1) {
+        if (p.part_num == nullptr) {
           p.out_max[orow] = final_max(m_true, l, p.scale_div);
           p.out_sum[orow] = l * f;
         } else {
@@ -921,7 +921,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) fwd_pair_kernel(const FwdParams
         if (!(ok = wait_warp(bar(kVFree0 + gl % kVStages), (gl / kVStages) & 1u, abort_flag))) break;
         tc_fence_after();
         const size_t orow = (size_t)w.token * kPrHeads + row;
-        if (p.split == 1) {
+        if (p.part_num == nullptr) {
           // O * (1/l) with the correctly rounded reciprocal (within an FP32 ulp of
           // O / l); a row without a valid index (l == 0) is written as 0
           const float rl = lf.x > 0.f ? __frcp_rn(lf.x) : 0.f;

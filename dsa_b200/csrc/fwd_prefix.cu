@@ -1,0 +1,738 @@
+// tcgen05 attention of every query row over one dense key range that all of
+// them share (a common prompt), and the join with partials over each query's
+// own selected keys.
+//
+// Every (query, head) pair is a row, whatever query it belongs to: 128 rows
+// are one MMA tile, and the keys need no gather. A cluster of two CTAs owns
+// one item (row tile, key split) and walks its keys in tiles of 64:
+//
+//   score CTA (rank 0)  S = Q . K^T    M=128 rows, N=64 keys, K=576, Q in TMEM
+//                       P = bf16(exp(S / scale_div - m)), online softmax
+//   value CTA (rank 1)  O += P . V     M=128, N=2x256, K=64 keys, O fills TMEM
+//
+// O takes all 512 TMEM columns of an SM and Q 288 of another, as in the pair
+// family, whose split of the work and lazy rescale (the factor is applied only
+// when a row's maximum grows by more than 2^8) this kernel keeps.
+//
+// Keys come by TMA (one 3-D map that turns a row of 512 into eight 64-wide
+// blocks, 128-byte swizzle): 8 KB blocks of 64 keys x 64 dims in a ring of 20
+// in the score CTA, each released by the four MMAs that read it, and 32 KB
+// half tiles (64 keys x 256 columns) in a ring of 5 in the value CTA. Fine
+// slots keep more bytes in flight than whole tiles do: a tile is 72 KB.
+//
+// P rounds the weights to BF16 for the MMA; the row sum adds them before the
+// rounding, in FP32 (as every other family here).
+//
+// Roles (12 warps): score CTA 0 TMA, 1 QK issuer, 2 P sender, 4-11 softmax
+// (warps 4-7 the even, 8-11 the odd tiles; the running maximum goes from one
+// to the other); value CTA 0 TMA, 1 PV issuer, 4-11 rescale and epilogue.
+// Every wait is bounded and reports through the status word. No multicast
+// loads.
+#include <cuda.h>
+
+#include "prefix.cuh"
+#include "umma_ptx.cuh"
+
+namespace dsa {
+namespace {
+
+using namespace umma;
+
+constexpr int kPxThreads = 384;
+constexpr int kPxRows = 128;
+constexpr uint32_t kBlk = 64u * 128u;        // 64 keys x 64 dims, SW128
+constexpr uint32_t kHalf = 4u * kBlk;        // 64 keys x 256 value columns
+constexpr int kKSlots = 20;                  // score CTA: ring of K blocks
+constexpr int kVSlots = 5;                   // value CTA: ring of V half tiles
+constexpr int kSBufs = 3;
+constexpr int kPSlots = 3;                   // value CTA
+constexpr int kLSlots = 2;                   // score CTA: P staging (slot g % 2 is softmax group g % 2's)
+constexpr uint32_t kPBytes = 128u * 64u * 2u;
+constexpr uint32_t kAlphaOff = kPBytes;
+constexpr uint32_t kFlagOff = kPBytes + 512u;
+constexpr uint32_t kMsgBytes = kPBytes + 512u + 16u;
+constexpr uint32_t kSlotBytes = kPBytes + 1024u;
+constexpr uint32_t kFinBytes = 128u * 8u;
+constexpr int kSoftWarp0 = 4;
+constexpr int kEpiWarps = 8;
+
+enum Bar {
+  kKFull0 = 0,
+  kKFree0 = kKFull0 + kKSlots,
+  kQFull = kKFree0 + kKSlots,
+  kSFull0,
+  kSFree0 = kSFull0 + kSBufs,
+  kMReady0 = kSFree0 + kSBufs,      // 4: per lane quadrant, the running max of the latest tile is posted
+  kXchg0 = kMReady0 + 4,            // 4: per lane quadrant, both softmax warps posted their totals
+  kLFull0 = kXchg0 + 4,             // P staging slot written (4 warps)
+  kLFree0 = kLFull0 + kLSlots,      // P staging slot's message has landed (arrive from the value CTA)
+  kPDone0 = kLFree0 + kLSlots,      // PV that read the P slot is done (commit to both CTAs)
+  kVFull0 = kPDone0 + kPSlots,
+  kVFree0 = kVFull0 + kVSlots,
+  kPFull0 = kVFree0 + kVSlots,      // P message landed
+  kReq = kPFull0 + kPSlots,         // a rescale request is posted
+  kReqDone,
+  kFin,                             // (l, f) landed
+  kDrain,                           // abort path: issued MMAs are done
+  kBarCount
+};
+constexpr uint32_t kOffTmemSlot = kBarCount * 8u;
+constexpr uint32_t kOffAbort = kOffTmemSlot + 8u;
+constexpr uint32_t kOffReq = kOffAbort + 8u;
+constexpr uint32_t kOffData = 1024u;
+constexpr uint32_t kOffLocal = kOffData + kKSlots * kBlk;          // score CTA
+constexpr uint32_t kOffM = kOffLocal + kLSlots * kSlotBytes;       // [2][4 quads][32] running maxima
+constexpr uint32_t kOffX = kOffM + 2u * 4u * 32u * 4u;             // [4 quads][2 warps][3][32] totals
+constexpr uint32_t kScoreBytes = kOffX + 4u * 2u * 3u * 32u * 4u;
+constexpr uint32_t kOffSlot = kOffData + kVSlots * kHalf;          // value CTA
+constexpr uint32_t kOffFin = kOffSlot + kPSlots * kSlotBytes;
+constexpr uint32_t kValueBytes = kOffFin + kFinBytes;
+constexpr uint32_t kSmemBytes = (kScoreBytes > kValueBytes ? kScoreBytes : kValueBytes) + 1024u;
+constexpr uint32_t kReqEnd = 0xffffffffu;
+constexpr uint32_t kTmemCols = 512, kTmemQ = 0, kTmemS = 288, kTmemO = 0;
+
+static_assert(kOffReq + 8u <= kOffData, "barrier block");
+static_assert(kOffLocal % 1024 == 0 && kOffSlot % 1024 == 0 && kSlotBytes % 1024 == 0, "swizzle atoms");
+static_assert(kSmemBytes <= 232448, "shared memory budget");
+static_assert(kTmemS + kSBufs * 64 <= kTmemCols, "score TMEM budget");
+
+__device__ __forceinline__ float u2f(uint32_t v) { return __uint_as_float(v); }
+__device__ __forceinline__ uint32_t f2u(float v) { return __float_as_uint(v); }
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, volatile int* abort,
+                                          bool cluster_scope = false) {
+  const bool ok = mbar_wait(bar, parity, abort, cluster_scope);
+  return __all_sync(0xffffffffu, ok) != 0;
+}
+__device__ __forceinline__ void st_async_b32x2(uint32_t remote_addr, uint32_t remote_bar, uint32_t a, uint32_t b) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.b32 [%0], {%1, %2}, [%3];" ::"r"(
+                   remote_addr),
+               "r"(a), "r"(b), "r"(remote_bar)
+               : "memory");
+}
+__device__ __forceinline__ void mma_commit_mc(uint32_t bar, uint16_t cta_mask) {
+  asm volatile(
+      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          bar),
+      "h"(cta_mask)
+      : "memory");
+}
+// Box of the map at (0, row, blk) -> shared memory of this CTA.
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int row, int blk, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          dst),
+      "l"(map), "r"(0), "r"(row), "r"(blk), "r"(bar)
+      : "memory");
+}
+
+struct Maps {
+  CUtensorMap k;     // latent, boxes of 64 keys x 64 dims
+  CUtensorMap v;     // latent, boxes of 64 keys x 256 dims
+  CUtensorMap rope;  // rope, boxes of 64 keys x 64 dims
+};
+
+// Chunk `ch` (dims 64ch..; 8: rope) of one Q row -> 32 TMEM columns of this lane.
+__device__ __forceinline__ void load_q_chunk(const PrefixParams& p, size_t row, int ch, uint32_t taddr) {
+  const uint4* s4 = ch < 8 ? reinterpret_cast<const uint4*>(p.q + row * kDimLatent) + ch * 8
+                           : reinterpret_cast<const uint4*>(p.q_rope + row * kDimRope);
+  uint32_t r[32];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const uint4 v = __ldg(s4 + k);
+    r[4 * k] = v.x;
+    r[4 * k + 1] = v.y;
+    r[4 * k + 2] = v.z;
+    r[4 * k + 3] = v.w;
+  }
+  tmem_st32(taddr, r);
+}
+
+__global__ void __launch_bounds__(kPxThreads, 1) fwd_prefix_kernel(const PrefixParams p,
+                                                                   const __grid_constant__ Maps maps) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* const sbase = smem_raw + (base - raw);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const int item = (int)(blockIdx.x >> 1);
+  const int mt = item / p.split, sp = item - mt * p.split;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(sbase + kOffAbort);
+  auto bar = [&](int i) -> uint32_t { return base + 8u * (uint32_t)i; };
+
+  // keys [tile0 * 64, ...) of the split: whole tiles of the keys in use
+  const int used = p.length != nullptr ? min(max(__ldg(p.length), 0), p.keys) : p.keys;
+  const int all_tiles = (used + 63) / 64;
+  const int tile0 = (int)((long long)all_tiles * sp / p.split);
+  const int ntiles = (int)((long long)all_tiles * (sp + 1) / p.split) - tile0;
+  const bool direct = p.part_num == nullptr;
+  const long long row0 = (long long)mt * kPxRows;
+
+  if (ntiles == 0) {  // the same in both CTAs: nothing to attend to
+    for (int r = threadIdx.x; r < kPxRows; r += kPxThreads) {
+      if (rank == 0 && direct && row0 + r < p.rows) {
+        p.out_max[row0 + r] = -INFINITY;
+        p.out_sum[row0 + r] = 0.f;
+      } else if (rank == 0 && !direct) {
+        p.part_max[(size_t)item * kPxRows + r] = kNegFltMax;
+        p.part_sum[(size_t)item * kPxRows + r] = 0.f;  // the join does not read the numerator then
+      }
+    }
+    if (rank == 1 && direct)
+      for (int c = threadIdx.x; c < kPxRows * 64; c += kPxThreads)
+        if (row0 + (c >> 6) < p.rows)
+          reinterpret_cast<uint4*>(p.out + (row0 + (c >> 6)) * kDimLatent)[c & 63] = make_uint4(0, 0, 0, 0);
+    return;
+  }
+
+  if (threadIdx.x == 0) {
+    if (rank == 0) {
+      for (int s = 0; s < kKSlots; ++s) {
+        mbar_init(bar(kKFull0 + s), 1);
+        mbar_init(bar(kKFree0 + s), 1);
+      }
+      mbar_init(bar(kQFull), 8);
+      for (int i = 0; i < kSBufs; ++i) {
+        mbar_init(bar(kSFull0 + i), 1);
+        mbar_init(bar(kSFree0 + i), 4);
+      }
+      for (int q = 0; q < 4; ++q) {
+        mbar_init(bar(kMReady0 + q), 1);
+        mbar_init(bar(kXchg0 + q), 2);
+      }
+      for (int s = 0; s < kLSlots; ++s) {
+        mbar_init(bar(kLFull0 + s), 4);
+        mbar_init(bar(kLFree0 + s), 1);
+      }
+    } else {
+      for (int s = 0; s < kVSlots; ++s) {
+        mbar_init(bar(kVFull0 + s), 1);
+        mbar_init(bar(kVFree0 + s), 1);
+      }
+      for (int s = 0; s < kPSlots; ++s) mbar_init(bar(kPFull0 + s), 1);
+      mbar_init(bar(kReq), 1);
+      mbar_init(bar(kReqDone), kEpiWarps);
+      mbar_init(bar(kFin), 1);
+    }
+    for (int s = 0; s < kPSlots; ++s) mbar_init(bar(kPDone0 + s), 1);
+    mbar_init(bar(kDrain), 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 0) {
+    tmem_alloc(base + kOffTmemSlot, kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(sbase + kOffTmemSlot);
+  if (rank == 1 && threadIdx.x == 0) {
+    for (int s = 0; s < kPSlots; ++s) mbar_arrive_expect_tx(bar(kPFull0 + s), kMsgBytes);
+    mbar_arrive_expect_tx(bar(kFin), kFinBytes);
+  }
+  cluster_sync();
+
+  bool ok = true;
+  if (rank == 0) {
+    // =============================== score CTA ===============================
+    if (warp == 0) {
+      // ---- TMA: block n = 9 t + j of the item's K blocks into slot n % kKSlots ----
+      const int total = 9 * ntiles;
+      int n = 0;
+      for (int t = 0; t < ntiles && ok; ++t) {
+        for (int j = 0; j < 9; ++j, ++n) {
+          const uint32_t s = (uint32_t)n % kKSlots;
+          if (n >= kKSlots && !(ok = wait_warp(bar(kKFree0 + s), (uint32_t)(n / kKSlots - 1) & 1u, abort_flag))) break;
+          if (elect_one()) {
+            mbar_arrive_expect_tx(bar(kKFull0 + s), kBlk);
+            tma_load_3d(base + kOffData + s * kBlk, j < 8 ? &maps.k : &maps.rope, (tile0 + t) * 64, j < 8 ? j : 0,
+                        bar(kKFull0 + s));
+          }
+          __syncwarp();
+        }
+      }
+      if (!ok)  // loads in flight land before the CTA's memory goes
+        for (int k = max(0, n - kKSlots); k < n && k < total; ++k)
+          mbar_wait_drain(bar(kKFull0 + k % kKSlots), (uint32_t)(k / kKSlots) & 1u);
+    } else if (warp == 1) {
+      // ---- QK issuer: S buffer g % 3 <- Q . K^T, block by block ----
+      const uint32_t idesc = idesc_bf16(128, 64, false, false);
+      ok = wait_warp(bar(kQFull), 0u, abort_flag);
+      tc_fence_after();
+      int n = 0;
+      for (int g = 0; g < ntiles && ok; ++g) {
+        const uint32_t b = (uint32_t)g % kSBufs;
+        if (g >= kSBufs && !(ok = wait_warp(bar(kSFree0 + b), (uint32_t)(g / kSBufs - 1) & 1u, abort_flag))) break;
+        const uint32_t d = tmem + kTmemS + b * 64u;
+        for (int j = 0; j < 9; ++j, ++n) {
+          const uint32_t s = (uint32_t)n % kKSlots;
+          if (!(ok = wait_warp(bar(kKFull0 + s), (uint32_t)(n / kKSlots) & 1u, abort_flag))) break;
+          tc_fence_after();
+          const uint32_t slot = base + kOffData + s * kBlk;
+          if (elect_one()) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              mma_bf16_ts(d, tmem + kTmemQ + (uint32_t)(j * 4 + k) * 8u,
+                          smem_desc(slot + (uint32_t)k * 32u, 16, 1024, kLayoutSw128), idesc, (j | k) ? 1u : 0u);
+            mma_commit(bar(kKFree0 + s));
+            if (j == 8) mma_commit(bar(kSFull0 + b));
+          }
+          __syncwarp();
+        }
+      }
+      if (!ok) {
+        if (elect_one()) mma_commit(bar(kDrain));
+        __syncwarp();
+        mbar_wait_drain(bar(kDrain), 0u);
+      }
+    } else if (warp == 2) {
+      // ---- P sender: staging slot g % 2 -> the value CTA's P slot g % 3 ----
+      const uint32_t r_slot0 = mapa_shared(base + kOffSlot, 1);
+      const uint32_t r_pfull0 = mapa_shared(bar(kPFull0), 1);
+      int g = 0;
+      for (; g < ntiles; ++g) {
+        const uint32_t ls = (uint32_t)g % kLSlots, ps = (uint32_t)g % kPSlots;
+        if (!(ok = wait_warp(bar(kLFull0 + ls), (uint32_t)(g / kLSlots) & 1u, abort_flag))) break;
+        if (g >= kPSlots && !(ok = wait_warp(bar(kPDone0 + ps), (uint32_t)(g / kPSlots - 1) & 1u, abort_flag))) break;
+        if (lane == 0)
+          bulk_copy_to_peer(r_slot0 + ps * kSlotBytes, base + kOffLocal + ls * kSlotBytes, kMsgBytes,
+                            r_pfull0 + 8u * ps);
+        __syncwarp();
+      }
+      // the value CTA's last commits arrive in this CTA's memory
+      for (int k = max(0, ntiles - kPSlots); k < ntiles && ok; ++k)
+        ok = wait_warp(bar(kPDone0 + k % kPSlots), (uint32_t)(k / kPSlots) & 1u, abort_flag);
+    } else if (warp >= kSoftWarp0) {
+      // ---- softmax: one row per thread; group e takes tiles g % 2 == e ----
+      const int quad = warp & 3;
+      const int e = (warp - kSoftWarp0) >> 2;
+      const int row = quad * 32 + lane;
+      const uint32_t t_lane = (uint32_t)(quad * 32) << 16;
+      const float c = p.scale_log2;
+      float* const mpub = reinterpret_cast<float*>(sbase + kOffM);
+      float* const xch = reinterpret_cast<float*>(sbase + kOffX);
+      {
+        const size_t qrow = (size_t)min(row0 + row, p.rows - 1);  // rows past the end repeat the last one
+        const uint32_t tq = tmem + t_lane + kTmemQ;
+#pragma unroll 1
+        for (int ch = e * 5; ch < (e == 0 ? 5 : 9); ++ch) load_q_chunk(p, qrow, ch, tq + (uint32_t)ch * 32u);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(kQFull));
+      }
+      float m_w = kNegFltMax, m_true = kNegFltMax, l = 0.f;
+      for (int g = e; g < ntiles; g += 2) {
+        const uint32_t b = (uint32_t)g % kSBufs;
+        if (!(ok = wait_warp(bar(kSFull0 + b), (uint32_t)(g / kSBufs) & 1u, abort_flag))) break;
+        tc_fence_after();
+        float x[64];
+        {
+          uint32_t sv[64];
+          tmem_ld32(tmem + t_lane + kTmemS + b * 64u, sv);
+          tmem_ld32(tmem + t_lane + kTmemS + b * 64u + 32u, sv + 32);
+          tmem_wait_ld_regs32(sv);
+          tmem_wait_ld_regs32(sv + 32);
+#pragma unroll
+          for (int k = 0; k < 64; ++k) x[k] = u2f(sv[k]);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(kSFree0 + b));
+        const int valid = used - (tile0 + g) * 64;
+        if (valid < 64) {
+#pragma unroll
+          for (int k = 0; k < 64; ++k) x[k] = k < valid ? x[k] : -INFINITY;
+        }
+        float mx;
+        {
+          float r[32];
+#pragma unroll
+          for (int k = 0; k < 32; ++k) r[k] = fmaxf(x[k], x[k + 32]);
+#pragma unroll
+          for (int w = 16; w >= 1; w >>= 1)
+#pragma unroll
+            for (int k = 0; k < w; ++k) r[k] = fmaxf(r[k], r[k + w]);
+          mx = r[0];
+        }
+        m_true = fmaxf(m_true, mx);
+        float m_prev = kNegFltMax;
+        if (g > 0) {
+          if (!(ok = wait_warp(bar(kMReady0 + quad), (uint32_t)(g - 1) & 1u, abort_flag))) break;
+          m_prev = mpub[(((g - 1) & 1) * 4 + quad) * 32 + lane];
+        }
+        const float m_t = ((mx - m_prev) * c > 8.f) ? mx : m_prev;  // lazy rescale threshold 2^8
+        mpub[((g & 1) * 4 + quad) * 32 + lane] = m_t;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(kMReady0 + quad));
+        const bool resc = g > 0 && m_t != m_prev;  // the first PV overwrites O
+        const float alpha = resc ? ex2((m_prev - m_t) * c) : 1.f;
+        const float mc = m_t * c;
+        uint32_t packed[32];
+        float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+#pragma unroll
+        for (int k = 0; k < 64; k += 4) {
+          const float p0 = ex2(fmaf(x[k], c, -mc)), p1 = ex2(fmaf(x[k + 1], c, -mc));
+          const float p2 = ex2(fmaf(x[k + 2], c, -mc)), p3 = ex2(fmaf(x[k + 3], c, -mc));
+          s0 += p0;
+          s1 += p1;
+          s2 += p2;
+          s3 += p3;
+          packed[k / 2] = pack_bf16x2(p0, p1);
+          packed[k / 2 + 1] = pack_bf16x2(p2, p3);
+        }
+        if (m_t != m_w) {
+          l *= ex2((m_w - m_t) * c);
+          m_w = m_t;
+        }
+        l += (s0 + s1) + (s2 + s3);
+        const uint32_t flag = __any_sync(0xffffffffu, resc) ? 1u : 0u;
+        // the staging slot's message of tile g - 2 has landed
+        if (g >= kLSlots && !(ok = wait_warp(bar(kLFree0 + e), (uint32_t)(g / kLSlots - 1) & 1u, abort_flag, true))) break;
+        uint8_t* const slot = sbase + kOffLocal + (uint32_t)e * kSlotBytes;
+        uint8_t* const prow = slot + (uint32_t)(row >> 3) * 1024u + (uint32_t)(row & 7) * 128u;
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+          *reinterpret_cast<uint4*>(prow + (uint32_t)((q ^ (row & 7)) * 16)) =
+              make_uint4(packed[4 * q], packed[4 * q + 1], packed[4 * q + 2], packed[4 * q + 3]);
+        *reinterpret_cast<float*>(slot + kAlphaOff + (uint32_t)row * 4u) = alpha;
+        if (lane == 0) *reinterpret_cast<uint32_t*>(slot + kFlagOff + (uint32_t)quad * 4u) = flag;
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(kLFull0 + e));
+      }
+      // ---- totals of the two groups ----
+      if (ok) {
+        float* const mine = xch + (quad * 2 + e) * 96;
+        const float* const other = xch + (quad * 2 + (e ^ 1)) * 96;
+        mine[lane] = m_w;
+        mine[32 + lane] = l;
+        mine[64 + lane] = m_true;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(kXchg0 + quad));
+        ok = wait_warp(bar(kXchg0 + quad), 0u, abort_flag);
+        if (ok && e == 0) {
+          const float m_o = other[lane], l_o = other[32 + lane];
+          const float m_fin = fmaxf(m_w, m_o);
+          l = (m_w == m_fin ? l : l * ex2((m_w - m_fin) * c)) + (m_o == m_fin ? l_o : l_o * ex2((m_o - m_fin) * c));
+          m_true = fmaxf(m_true, other[64 + lane]);
+          const float f = m_true == kNegFltMax ? 1.f : ex2((m_fin - m_true) * c);
+          if (!direct) {
+            const size_t pr = (size_t)item * kPxRows + row;
+            p.part_max[pr] = m_true == kNegFltMax ? kNegFltMax : __fdiv_rn(m_true, p.scale_div);
+            p.part_sum[pr] = l * f;
+          } else if (row0 + row < p.rows) {
+            p.out_max[row0 + row] = final_max(m_true, l, p.scale_div);
+            p.out_sum[row0 + row] = l * f;
+          }
+          st_async_b32x2(mapa_shared(base + kOffFin, 1) + (uint32_t)row * 8u, mapa_shared(bar(kFin), 1), f2u(l), f2u(f));
+        }
+      }
+    }
+  } else {
+    // =============================== value CTA ===============================
+    if (warp == 0) {
+      // ---- TMA: half tile n = 2 t + h into slot n % kVSlots ----
+      int n = 0;
+      for (; n < 2 * ntiles; ++n) {
+        const uint32_t s = (uint32_t)n % kVSlots;
+        if (n >= kVSlots && !(ok = wait_warp(bar(kVFree0 + s), (uint32_t)(n / kVSlots - 1) & 1u, abort_flag))) break;
+        if (elect_one()) {
+          mbar_arrive_expect_tx(bar(kVFull0 + s), kHalf);
+          tma_load_3d(base + kOffData + s * kHalf, &maps.v, (tile0 + (n >> 1)) * 64, (n & 1) * 4, bar(kVFull0 + s));
+        }
+        __syncwarp();
+      }
+      if (!ok)
+        for (int k = max(0, n - kVSlots); k < n; ++k)
+          mbar_wait_drain(bar(kVFull0 + k % kVSlots), (uint32_t)(k / kVSlots) & 1u);
+    } else if (warp == 1) {
+      // ---- PV issuer ----
+      const uint32_t idesc = idesc_bf16(128, 256, false, true);
+      volatile uint32_t* const req = reinterpret_cast<volatile uint32_t*>(sbase + kOffReq);
+      const uint32_t r_lfree0 = mapa_shared(bar(kLFree0), 0);
+      uint32_t nresc = 0;
+      for (int g = 0; g < ntiles && ok; ++g) {
+        const uint32_t s = (uint32_t)g % kPSlots;
+        if (!(ok = wait_warp(bar(kPFull0 + s), (uint32_t)(g / kPSlots) & 1u, abort_flag, true))) break;
+        const uint32_t slot = base + kOffSlot + s * kSlotBytes;
+        if (elect_one()) {
+          mbar_arrive_remote(r_lfree0 + 8u * ((uint32_t)g % kLSlots));          // the staging slot may be written again
+          if (g + kPSlots < ntiles) mbar_arrive_expect_tx(bar(kPFull0 + s), kMsgBytes);  // its next message
+        }
+        __syncwarp();
+        const volatile uint32_t* fl = reinterpret_cast<const volatile uint32_t*>(sbase + (slot - base) + kFlagOff);
+        if ((fl[0] | fl[1] | fl[2] | fl[3]) != 0u) {
+          if (elect_one()) {
+            *req = (uint32_t)g;
+            mbar_arrive(bar(kReq));
+          }
+          __syncwarp();
+          if (!(ok = wait_warp(bar(kReqDone), nresc & 1u, abort_flag))) break;
+          ++nresc;
+        }
+        const int valid = used - (tile0 + g) * 64;
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) {
+          const int n = 2 * g + h;
+          const uint32_t vs = (uint32_t)n % kVSlots;
+          if (!(ok = wait_warp(bar(kVFull0 + vs), (uint32_t)(n / kVSlots) & 1u, abort_flag))) break;
+          const uint32_t vslot = base + kOffData + vs * kHalf;
+          if (valid < 64) {
+            // rows behind the last key: weight 0, but 0 x NaN of a cache row never written would not be 0
+            for (int i = lane; i < (64 - valid) * 32; i += 32) {
+              const int r = valid + (i >> 5), q = i & 31;
+              *reinterpret_cast<uint4*>(sbase + (vslot - base) + (uint32_t)(q >> 3) * kBlk + (uint32_t)r * 128u +
+                                        (uint32_t)(q & 7) * 16u) = make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+          tc_fence_after();
+          if (elect_one()) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              mma_bf16_ss(tmem + kTmemO + h * 256, smem_desc(slot + j * 32, 16, 1024, kLayoutSw128),
+                          smem_desc(vslot + j * 2048, kBlk, 1024, kLayoutSw128), idesc, (g | j) ? 1u : 0u);
+            mma_commit(bar(kVFree0 + vs));
+            if (h == 1) mma_commit_mc(bar(kPDone0 + s), (uint16_t)3);
+          }
+          __syncwarp();
+        }
+      }
+      if (ok) {
+        if (elect_one()) {
+          *req = kReqEnd;
+          mbar_arrive(bar(kReq));
+        }
+        __syncwarp();
+      } else {
+        if (elect_one()) mma_commit(bar(kDrain));
+        __syncwarp();
+        mbar_wait_drain(bar(kDrain), 0u);
+      }
+    } else if (warp >= kSoftWarp0) {
+      // ---- rescale requests, then the epilogue: half `part` of the columns of 32 rows ----
+      const int quad = warp & 3, part = (warp - kSoftWarp0) >> 2;
+      const int row = quad * 32 + lane;
+      const uint32_t t_o = tmem + ((uint32_t)(quad * 32) << 16) + kTmemO + (uint32_t)part * 256u;
+      const volatile uint32_t* const req = reinterpret_cast<const volatile uint32_t*>(sbase + kOffReq);
+      auto pv_done = [&](int g) { return wait_warp(bar(kPDone0 + g % kPSlots), (uint32_t)(g / kPSlots) & 1u, abort_flag); };
+      for (uint32_t nreq = 0;; ++nreq) {
+        if (!(ok = wait_warp(bar(kReq), nreq & 1u, abort_flag))) break;
+        const uint32_t g = *req;
+        if (g == kReqEnd) break;
+        const uint8_t* slot = sbase + kOffSlot + (g % kPSlots) * kSlotBytes;
+        const uint32_t flag = *reinterpret_cast<const volatile uint32_t*>(slot + kFlagOff + quad * 4);
+        if (flag != 0u) {
+          const float alpha = *reinterpret_cast<const volatile float*>(slot + kAlphaOff + row * 4);
+          if (!(ok = pv_done((int)g - 1))) break;
+          tc_fence_after();
+#pragma unroll 1
+          for (int cb = 0; cb < 256; cb += 32) {
+            uint32_t o[32];
+            tmem_ld32(t_o + (uint32_t)cb, o);
+            tmem_wait_ld_regs32(o);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) o[k] = f2u(u2f(o[k]) * alpha);
+            tmem_st32(t_o + (uint32_t)cb, o);
+          }
+          tmem_wait_st();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(kReqDone));
+      }
+      if (ok && (ok = wait_warp(bar(kFin), 0u, abort_flag, true)) && (ok = pv_done(ntiles - 1))) {
+        const volatile float* lf = reinterpret_cast<const volatile float*>(sbase + kOffFin + row * 8);
+        const float l = lf[0], f = lf[1];
+        tc_fence_after();
+        const long long grow = row0 + row;
+        if (direct) {
+          const float rl = l > 0.f || l != l ? __frcp_rn(l) : 0.f;
+          __nv_bfloat16* const dst = p.out + (size_t)(grow & ~1LL) * kDimLatent + part * 256;
+          const bool wide = (reinterpret_cast<uintptr_t>(p.out) & 31u) == 0;
+#pragma unroll 1
+          for (int cb = 0; cb < 256; cb += 32) {
+            uint32_t o[32];
+            tmem_ld32(t_o + (uint32_t)cb, o);
+            tmem_wait_ld_regs32(o);
+            uint32_t a[8], b[8];
+            pack_bf16_row32_paired(o, rl, a, b);
+            if (grow < p.rows) store_bf16_row32_paired(dst + cb, kDimLatent, a, b, wide);  // rows is even: pairs are whole
+          }
+        } else {
+          float* const dst = p.part_num + ((size_t)item * kPxRows + row) * kDimLatent + part * 256;
+#pragma unroll 1
+          for (int cb = 0; cb < 256; cb += 32) {
+            uint32_t o[32];
+            tmem_ld32(t_o + (uint32_t)cb, o);
+            tmem_wait_ld_regs32(o);
+            if (grow < p.rows) store_f32_row32(dst + cb, o, f, true);
+          }
+        }
+        tc_fence_before();
+      }
+    }
+  }
+  if (!ok && lane == 0) report_error(p.status, kErrTimeout);
+  __syncwarp();
+  tc_fence_before();
+  cluster_sync();
+  if (warp == 0) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+// Join of a row's prefix partials and its own-key partials: m = max m_i,
+// out = sum_i e^(m_i - m) n_i / sum_i e^(m_i - m) l_i. One warp per row, a
+// lane's columns are 4 lane + 128 k; parts with sum 0 are not read.
+__global__ void __launch_bounds__(256) prefix_join_kernel(const JoinParams p) {
+  const int lane = threadIdx.x & 31;
+  const long long r = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (r >= p.rows) return;
+  const long long mt = r >> 7;
+  const int n = p.split + p.own_split;
+  const long long token = r / p.heads;
+  auto at = [&](int i, const float*& num, float& m, float& l) {
+    if (i < p.split) {
+      const size_t k = (size_t)(mt * p.split + i) * kPxRows + (size_t)(r & 127);
+      num = p.part_num + k * kDimLatent;
+      m = p.part_max[k];
+      l = p.part_sum[k];
+    } else {
+      const size_t k = ((size_t)token * p.own_split + (i - p.split)) * p.heads + (size_t)(r - token * p.heads);
+      num = p.own_num + k * kDimLatent;
+      m = p.own_max[k];
+      l = p.own_sum[k];
+    }
+  };
+  float top = kNegFltMax;
+  for (int i = 0; i < n; ++i) {
+    const float* num;
+    float m, l;
+    at(i, num, m, l);
+    if (l != 0.f) top = fmaxf(top, m);
+  }
+  float4 acc[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+  float total = 0.f;
+  for (int i = 0; i < n; ++i) {
+    const float* num;
+    float m, l;
+    at(i, num, m, l);
+    if (l == 0.f) continue;
+    const float w = expf(m - top);
+    total += w * l;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float4 v = *reinterpret_cast<const float4*>(num + 4 * lane + 128 * k);
+      acc[k].x = fmaf(w, v.x, acc[k].x);
+      acc[k].y = fmaf(w, v.y, acc[k].y);
+      acc[k].z = fmaf(w, v.z, acc[k].z);
+      acc[k].w = fmaf(w, v.w, acc[k].w);
+    }
+  }
+  const float rl = total != 0.f ? __frcp_rn(total) : 0.f;
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    *reinterpret_cast<uint2*>(p.out + r * kDimLatent + 4 * lane + 128 * k) =
+        make_uint2(pack_bf16x2(acc[k].x * rl, acc[k].y * rl), pack_bf16x2(acc[k].z * rl, acc[k].w * rl));
+  if (lane == 0) {
+    p.out_max[r] = total != 0.f ? top : -INFINITY;
+    p.out_sum[r] = total;
+  }
+}
+
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeFn encode_fn() {
+  static EncodeFn fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return reinterpret_cast<EncodeFn>(f);
+  }();
+  return fn;
+}
+
+// `rows` rows of blocks x 64 elements as [blocks][rows][64], boxes of
+// box_blocks x 64 rows x 64.
+bool encode(CUtensorMap* map, const void* ptr, long long rows, int blocks, int box_blocks) {
+  const EncodeFn fn = encode_fn();
+  if (fn == nullptr) return false;
+  const cuuint64_t dims[3] = {64, (cuuint64_t)rows, (cuuint64_t)blocks};
+  const cuuint64_t strides[2] = {(cuuint64_t)blocks * 128u, 128u};
+  const cuuint32_t box[3] = {64, 64, (cuuint32_t)box_blocks};
+  const cuuint32_t ones[3] = {1, 1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(ptr), dims, strides, box, ones,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool launch_config(cudaLaunchConfig_t* cfg, cudaLaunchAttribute* attr, unsigned ctas, cudaStream_t stream) {
+  if (cudaFuncSetAttribute(fwd_prefix_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes) != cudaSuccess)
+    return false;
+  attr->id = cudaLaunchAttributeClusterDimension;
+  attr->val.clusterDim.x = 2;
+  attr->val.clusterDim.y = 1;
+  attr->val.clusterDim.z = 1;
+  *cfg = cudaLaunchConfig_t{};
+  cfg->gridDim = dim3(ctas, 1, 1);
+  cfg->blockDim = dim3(kPxThreads, 1, 1);
+  cfg->dynamicSmemBytes = kSmemBytes;
+  cfg->stream = stream;
+  cfg->attrs = attr;
+  cfg->numAttrs = 1;
+  return true;
+}
+
+}  // namespace
+
+int prefix_max_clusters() {
+  static int cached = -1;
+  if (cached > 0) return cached;
+  cudaLaunchConfig_t cfg;
+  cudaLaunchAttribute attr;
+  int n = 0;
+  if (!launch_config(&cfg, &attr, 148, nullptr) ||
+      cudaOccupancyMaxActiveClusters(&n, fwd_prefix_kernel, &cfg) != cudaSuccess || n <= 0) {
+    cudaGetLastError();
+    return -1;
+  }
+  cached = n;
+  return cached;
+}
+
+cudaError_t launch_fwd_prefix(const PrefixParams& p, const void* kv, const void* k_rope, cudaStream_t stream) {
+  Maps maps;
+  if (!encode(&maps.k, kv, p.keys, 8, 1) || !encode(&maps.v, kv, p.keys, 8, 4) || !encode(&maps.rope, k_rope, p.keys, 1, 1))
+    return cudaErrorInvalidValue;
+  const long long items = (p.rows + kPxRows - 1) / kPxRows * p.split;
+  if (items <= 0 || 2 * items > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
+  cudaLaunchConfig_t cfg;
+  cudaLaunchAttribute attr;
+  if (!launch_config(&cfg, &attr, (unsigned)(2 * items), stream)) return cudaErrorInvalidConfiguration;
+  return cudaLaunchKernelEx(&cfg, fwd_prefix_kernel, p, maps);
+}
+
+cudaError_t launch_prefix_join(const JoinParams& p, cudaStream_t stream) {
+  prefix_join_kernel<<<(unsigned)((p.rows + 7) / 8), 256, 0, stream>>>(p);
+  return cudaGetLastError();
+}
+
+}  // namespace dsa

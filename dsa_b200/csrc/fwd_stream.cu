@@ -485,7 +485,7 @@ __global__ void __launch_bounds__(kStThreads, 2) fwd_stream_kernel(const FwdPara
 
     // ---- epilogue (sm.m / sm.l final after the last softmax barrier) ----
     const float l0 = sm.l[g], l1 = sm.l[g + 8];
-    if (p.split == 1) {
+    if (p.part_num == nullptr) {
       // a row without a valid index (l == 0, O == 0) is written as 0 (O / inf)
       const float d0 = l0 > 0.f ? l0 : INFINITY, d1 = l1 > 0.f ? l1 : INFINITY;
       __nv_bfloat16* o0 = p.out + ((size_t)w.token * p.heads + h0 + g) * kDimLatent + cw * 128 + tq * 2;
@@ -590,11 +590,11 @@ bool stream_cluster_merge(int split) {
   return cached[split] > 0;
 }
 
-cudaError_t launch_fwd_stream(const FwdParams& p, cudaStream_t stream) {
+cudaError_t launch_fwd_stream(const FwdParams& p, cudaStream_t stream, bool merge) {
   if (p.heads % kStHeads != 0 || p.keys_per_tile != kStBN) return cudaErrorInvalidValue;
   const long long items = (long long)p.tokens * (p.heads / kStHeads) * p.split;
   if (items <= 0 || items > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
-  if (p.split > 1 && stream_cluster_merge(p.split)) {
+  if (merge && p.split > 1 && stream_cluster_merge(p.split)) {
     cudaLaunchConfig_t cfg;
     cudaLaunchAttribute attr;
     st_cm_launch_config(&cfg, &attr, p.split, items, stream);

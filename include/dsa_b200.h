@@ -329,6 +329,29 @@ typedef struct dsa_append_kv_args {
 /* One kernel on `stream`. Returns a dsa_status_t. */
 DSA_B200_API int dsa_append_kv(const dsa_append_kv_args_t* args, void* stream);
 
+/* Dense keys that every query of a call attends to, next to its own selected
+ * keys (no counterpart in the reference). */
+typedef struct dsa_prefix_kv {
+  const void* kv;          /* BF16 [rows, 512] */
+  const void* k_rope;      /* BF16 [rows, 64] */
+  const int32_t* length;   /* device INT32 [1]: the first length rows are keys (clamped to [0, rows]); NULL: all */
+  int64_t rows;
+} dsa_prefix_kv_t;
+
+/* Workspace bytes of dsa_sparse_mla_fwd_prefix; 0 for invalid arguments, and
+ * where none is needed. */
+DSA_B200_API uint64_t dsa_fwd_prefix_workspace_bytes(const dsa_fwd_args_t* args, const dsa_prefix_kv_t* prefix);
+
+/* Forward of every query over the prefix keys and its own selected keys, as
+ * one softmax: q, q_rope, output and statistics as for dsa_sparse_mla_fwd;
+ * kv, k_rope, indices, length and topk describe each batch row's own keys, or
+ * are NULL / 0 for attention over the prefix alone. The prefix is read once
+ * per 128 (query, head) rows and split over the GPU; partials are joined in
+ * FP32. launch.family is AUTO. A row without any key gets output 0,
+ * softmax_max -inf, softmax_sum 0; prefix rows at and past the length do not
+ * matter, whatever they hold. Returns a dsa_status_t. */
+DSA_B200_API int dsa_sparse_mla_fwd_prefix(const dsa_fwd_args_t* args, const dsa_prefix_kv_t* prefix, void* stream);
+
 /* Number of kernels the last successful dsa_sparse_mla_fwd on this host
  * thread enqueued (1 or 2), for launch accounting. Calls of
  * dsa_sparse_mla_fwd_noalloc do not update it. */

@@ -1,0 +1,146 @@
+"""GPU parity of shared-prefix attention against its definition in FP64.
+
+Tolerances, with W = sum_j w_j |v_j| over a row's normalised weights and
+D = 2^-23 * 44 * max_j sum_i |q_i k_i| * scale, the bound of a score's error
+(36 accumulations of the MMA, each cut to FP32, and a few roundings of the
+scaling): a weight is off by a factor e^(+-2D) (its score and the maximum) and
+by half a BF16 step, 2^-8, for the MMA; the sum by e^(+-2D); the output rounds
+once more to BF16:
+  |out - ref| <= W (2^-8 + 5 D + 2^-18) + 2^-8 |ref|   (2^-18: exponentials, joins)
+  |max - ref| <= D + 2^-22 |ref|,  |sum - ref| <= ref (3 D + 2^-18)
+"""
+import pytest
+import torch
+
+import dsa_b200
+from dsa_b200 import shared_prefix
+
+pytestmark = pytest.mark.gpu
+
+
+def _reference(q, pk, qr, pr, kv, kr, ids, used, scale):
+    """FP64, query by query: (out, max, sum, W, D)."""
+    batch, queries, heads, _ = q.shape
+    key = torch.cat((pk, pr), -1)[0, :used, 0].double()
+    out = torch.zeros((batch, queries, heads, 512), dtype=torch.float64, device=q.device)
+    top = torch.full((batch, queries, heads), -float("inf"), dtype=torch.float64, device=q.device)
+    total, width, slack = torch.zeros_like(top), torch.zeros_like(out), torch.zeros_like(top)
+    for b in range(batch):
+        for s in range(queries):
+            keys = key
+            if ids is not None:
+                i = ids[b, s, 0].long()
+                i = i[(i >= 0) & (i < kv.shape[1])]
+                keys = torch.cat((key, torch.cat((kv[b, i, 0], kr[b, i, 0]), -1).double()))
+            if keys.shape[0] == 0:
+                continue
+            row = torch.cat((q[b, s], qr[b, s]), -1).double()
+            z = row @ keys.T * scale
+            top[b, s] = z.max(-1).values
+            w = torch.exp(z - top[b, s, :, None])
+            total[b, s] = w.sum(-1)
+            out[b, s] = w @ keys[:, :512] / total[b, s, :, None]
+            width[b, s] = w @ keys[:, :512].abs() / total[b, s, :, None]
+            slack[b, s] = (row.abs() @ keys.abs().T).max(-1).values * scale * 44 * 2.0 ** -23
+    return out, top, total, width, slack
+
+
+def _check(got, args, used, scale=1 / 24):
+    out, top, total, width, slack = _reference(*args, used, scale)
+    o, m, l = got[0].double(), got[1].double()[:, 0], got[2].double()[:, 0]
+    err = (o - out).abs() - (width * (2.0 ** -8 + 5 * slack[..., None] + 2.0 ** -18) + 2.0 ** -8 * out.abs())
+    assert float(err.max()) <= 0, float(err.max())
+    some = total > 0
+    assert bool((m[~some] == -float("inf")).all()) and bool((l[~some] == 0).all())
+    assert bool(((m - top).abs()[some] <= (slack + 2.0 ** -22 * top.abs())[some]).all())
+    assert bool(((l - total).abs()[some] <= (total * (3 * slack + 2.0 ** -18))[some]).all())
+    assert dsa_b200.device_status() == 0
+
+
+def _make(batch, queries, heads, prefix, length, topk, seed=1, gain=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+
+    def r(*shape):
+        return torch.randn(shape, generator=g, device="cuda").bfloat16()
+
+    q, qr = r(batch, queries, heads, 512) * gain, r(batch, queries, heads, 64) * gain
+    if not topk:
+        return q, r(1, prefix, 1, 512), qr, r(1, prefix, 1, 64), None, None, None
+    ids = torch.randint(0, length, (batch, queries, 1, topk), generator=g, device="cuda", dtype=torch.int32)
+    ids[torch.rand(ids.shape, generator=g, device="cuda") < 0.1] = -1
+    return q, r(1, prefix, 1, 512), qr, r(1, prefix, 1, 64), r(batch, length, 1, 512), r(batch, length, 1, 64), ids
+
+
+@pytest.mark.parametrize("gain", [1.0, 12.0])  # flat weights, and a few keys that take all: rescales
+@pytest.mark.parametrize("batch,queries,heads,prefix,length,topk", [
+    (1, 1, 16, 1, 0, 0), (1, 1, 16, 64, 0, 0), (2, 1, 128, 65, 0, 0), (1, 3, 48, 1000, 0, 0), (3, 2, 16, 1000, 300, 77),
+    (1, 1, 128, 129, 7, 1), (5, 7, 32, 4097, 50, 33), (64, 1, 16, 2048, 4096, 512), (9, 1, 128, 700, 2000, 2048),
+    (80, 1, 128, 200, 100, 64), (160, 1, 128, 130, 0, 0), (1, 1, 16, 30000, 1, 1), (2, 1, 144, 3000, 40, 40)])
+def test_parity(cuda_lib, batch, queries, heads, prefix, length, topk, gain):
+    args = _make(batch, queries, heads, prefix, length, topk, gain=gain)
+    _check(dsa_b200.forward_shared_prefix(*args), args, prefix)
+
+
+@pytest.mark.parametrize("topk", [0, 40])
+def test_filled_part(cuda_lib, topk):
+    """A buffer filled in part: lengths on every side of a tile's end, NaN and infinities behind the last key; one captured
+    graph serves all of them."""
+    args = _make(3, 2, 32, 700, 90, topk, seed=3)
+    if topk:
+        args[-1][1, 1] = -1  # a query without own keys
+    args[1][0, 130:] = float("nan")
+    args[3][0, 130:] = float("inf")
+    length = torch.zeros(1, dtype=torch.int32, device="cuda")
+    dsa_b200.forward_shared_prefix(*args, prefix_len=length)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = dsa_b200.forward_shared_prefix(*args, prefix_len=length)
+    for n in (0, 1, 63, 64, 65, 127, 128, 130, -5):
+        length.fill_(n)
+        graph.replay()
+        _check(got, args, max(n, 0))
+    args[1][0, 130:] = 1.0
+    args[3][0, 130:] = -1.0
+    for n in (131, 640, 699, 700, 100000):
+        length.fill_(n)
+        graph.replay()
+        _check(got, args, min(n, 700))
+
+
+def test_scale_and_repeat(cuda_lib):
+    args = _make(4, 3, 64, 5000, 300, 200, seed=5)
+    first = dsa_b200.forward_shared_prefix(*args, scale=0.11)
+    _check(first, args, 5000, 0.11)
+    again = dsa_b200.forward_shared_prefix(*args, scale=0.11)
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
+def test_in_pieces(cuda_lib, monkeypatch):
+    args = _make(3, 5, 16, 900, 60, 50, seed=6)
+    monkeypatch.setattr(shared_prefix, "WORKSPACE_BUDGET", 1 << 20)
+    _check(dsa_b200.forward_shared_prefix(*args), args, 900)
+
+
+def test_against_forward(cuda_lib):
+    """The same keys through ``forward``: prefix and own rows side by side, every index named."""
+    q, pk, qr, pr, kv, kr, ids = _make(2, 2, 128, 500, 300, 64, seed=7)
+    got = dsa_b200.forward_shared_prefix(q, pk, qr, pr, kv, kr, ids)
+    both = torch.cat((pk.expand(2, -1, -1, -1), kv), 1).contiguous(), torch.cat((pr.expand(2, -1, -1, -1), kr), 1).contiguous()
+    own = torch.where(ids >= 0, ids + 500, -1)
+    every = torch.cat((torch.arange(500, dtype=torch.int32, device="cuda").expand(2, 2, 1, 500), own), -1).contiguous()
+    ref = dsa_b200.forward(q, both[0], qr, both[1], every)
+    # two results of the bound above: twice 2^-8 (W <= ~1 here) and two BF16 roundings
+    assert float((got[0].float() - ref[0].float()).abs().max()) <= 4 * 2.0 ** -8
+    assert torch.allclose(got[1], ref[1], rtol=1e-5, atol=1e-5) and torch.allclose(got[2], ref[2], rtol=1e-4)
+
+
+def test_other_stream_and_unequal_calls_at_once(cuda_lib):
+    a, b = _make(2, 1, 16, 3000, 100, 64, seed=8), _make(1, 2, 128, 1500, 0, 0, seed=9)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        first = dsa_b200.forward_shared_prefix(*a)
+    second = dsa_b200.forward_shared_prefix(*b)
+    torch.cuda.synchronize()
+    _check(first, a, 3000)
+    _check(second, b, 1500)
