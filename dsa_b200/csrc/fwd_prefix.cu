@@ -15,10 +15,12 @@
 // when a row's maximum grows by more than 2^8) this kernel keeps.
 //
 // Keys come by TMA (one 3-D map that turns a row of 512 into eight 64-wide
-// blocks, 128-byte swizzle): 8 KB blocks of 64 keys x 64 dims in a ring of 20
-// in the score CTA, each released by the four MMAs that read it, and 32 KB
-// half tiles (64 keys x 256 columns) in a ring of 5 in the value CTA. Fine
-// slots keep more bytes in flight than whole tiles do: a tile is 72 KB.
+// blocks, 128-byte swizzle) in half tiles of 64 keys x 256 dims (32 KB), each
+// released by the MMAs that read it: a ring of 5 in the value CTA, two tiles
+// of two halves and a rope block in the score CTA. A box costs its issuer some
+// 300 cycles whatever its size, so 8 KB boxes cannot keep a tile's pace (nine
+// of them 3,200 cycles), and 32 KB ones can; whole tiles would keep fewer
+// bytes in flight.
 //
 // P rounds the weights to BF16 for the MMA; the row sum adds them before the
 // rounding, in FP32 (as every other family here).
@@ -42,11 +44,13 @@ constexpr int kPxThreads = 384;
 constexpr int kPxRows = 128;
 constexpr uint32_t kBlk = 64u * 128u;        // 64 keys x 64 dims, SW128
 constexpr uint32_t kHalf = 4u * kBlk;        // 64 keys x 256 value columns
-constexpr int kKSlots = 20;                  // score CTA: ring of K blocks
+constexpr int kKParts = 3;                   // score CTA: dims 0-255, 256-511 and rope of a tile
+constexpr int kKSlots = 2 * kKParts;         // two tiles
+constexpr uint32_t kKTile = 2u * kHalf + kBlk;
 constexpr int kVSlots = 5;                   // value CTA: ring of V half tiles
 constexpr int kSBufs = 3;
 constexpr int kPSlots = 3;                   // value CTA
-constexpr int kLSlots = 2;                   // score CTA: P staging (slot g % 2 is softmax group g % 2's)
+constexpr int kLSlots = 4;                   // score CTA: P staging (even: slot g % 4 is softmax group g % 2's)
 constexpr uint32_t kPBytes = 128u * 64u * 2u;
 constexpr uint32_t kAlphaOff = kPBytes;
 constexpr uint32_t kFlagOff = kPBytes + 512u;
@@ -65,8 +69,7 @@ enum Bar {
   kMReady0 = kSFree0 + kSBufs,      // 4: per lane quadrant, the running max of the latest tile is posted
   kXchg0 = kMReady0 + 4,            // 4: per lane quadrant, both softmax warps posted their totals
   kLFull0 = kXchg0 + 4,             // P staging slot written (4 warps)
-  kLFree0 = kLFull0 + kLSlots,      // P staging slot's message has landed (arrive from the value CTA)
-  kPDone0 = kLFree0 + kLSlots,      // PV that read the P slot is done (commit to both CTAs)
+  kPDone0 = kLFull0 + kLSlots,      // PV that read the P slot is done (commit to both CTAs)
   kVFull0 = kPDone0 + kPSlots,
   kVFree0 = kVFull0 + kVSlots,
   kPFull0 = kVFree0 + kVSlots,      // P message landed
@@ -80,7 +83,7 @@ constexpr uint32_t kOffTmemSlot = kBarCount * 8u;
 constexpr uint32_t kOffAbort = kOffTmemSlot + 8u;
 constexpr uint32_t kOffReq = kOffAbort + 8u;
 constexpr uint32_t kOffData = 1024u;
-constexpr uint32_t kOffLocal = kOffData + kKSlots * kBlk;          // score CTA
+constexpr uint32_t kOffLocal = kOffData + 2u * kKTile;              // score CTA
 constexpr uint32_t kOffM = kOffLocal + kLSlots * kSlotBytes;       // [2][4 quads][32] running maxima
 constexpr uint32_t kOffX = kOffM + 2u * 4u * 32u * 4u;             // [4 quads][2 warps][3][32] totals
 constexpr uint32_t kScoreBytes = kOffX + 4u * 2u * 3u * 32u * 4u;
@@ -133,8 +136,7 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
 }
 
 struct Maps {
-  CUtensorMap k;     // latent, boxes of 64 keys x 64 dims
-  CUtensorMap v;     // latent, boxes of 64 keys x 256 dims
+  CUtensorMap half;  // latent, boxes of 64 keys x 256 dims
   CUtensorMap rope;  // rope, boxes of 64 keys x 64 dims
 };
 
@@ -207,10 +209,7 @@ __global__ void __launch_bounds__(kPxThreads, 1) fwd_prefix_kernel(const PrefixP
         mbar_init(bar(kMReady0 + q), 1);
         mbar_init(bar(kXchg0 + q), 2);
       }
-      for (int s = 0; s < kLSlots; ++s) {
-        mbar_init(bar(kLFull0 + s), 4);
-        mbar_init(bar(kLFree0 + s), 1);
-      }
+      for (int s = 0; s < kLSlots; ++s) mbar_init(bar(kLFull0 + s), 4);
     } else {
       for (int s = 0; s < kVSlots; ++s) {
         mbar_init(bar(kVFull0 + s), 1);
@@ -244,46 +243,48 @@ __global__ void __launch_bounds__(kPxThreads, 1) fwd_prefix_kernel(const PrefixP
   if (rank == 0) {
     // =============================== score CTA ===============================
     if (warp == 0) {
-      // ---- TMA: block n = 9 t + j of the item's K blocks into slot n % kKSlots ----
-      const int total = 9 * ntiles;
-      int n = 0;
-      for (int t = 0; t < ntiles && ok; ++t) {
-        for (int j = 0; j < 9; ++j, ++n) {
-          const uint32_t s = (uint32_t)n % kKSlots;
-          if (n >= kKSlots && !(ok = wait_warp(bar(kKFree0 + s), (uint32_t)(n / kKSlots - 1) & 1u, abort_flag))) break;
-          if (elect_one()) {
-            mbar_arrive_expect_tx(bar(kKFull0 + s), kBlk);
-            tma_load_3d(base + kOffData + s * kBlk, j < 8 ? &maps.k : &maps.rope, (tile0 + t) * 64, j < 8 ? j : 0,
-                        bar(kKFull0 + s));
+      // ---- TMA: part j of tile t into slot 3 (t % 2) + j; one thread ----
+      if (lane == 0) {
+        int t = 0, j = 0;
+        for (; t < ntiles; ++t) {
+          const uint32_t s0 = (uint32_t)(t & 1) * kKParts, stage = base + kOffData + (uint32_t)(t & 1) * kKTile;
+          for (j = 0; j < kKParts; ++j) {
+            if (t >= 2 && !(ok = mbar_wait(bar(kKFree0 + s0 + j), (uint32_t)((t >> 1) - 1) & 1u, abort_flag))) break;
+            mbar_arrive_expect_tx(bar(kKFull0 + s0 + j), j < 2 ? kHalf : kBlk);
+            tma_load_3d(stage + (uint32_t)j * kHalf, j < 2 ? &maps.half : &maps.rope, (tile0 + t) * 64, j < 2 ? 4 * j : 0,
+                        bar(kKFull0 + s0 + j));
           }
-          __syncwarp();
+          if (!ok) break;
         }
+        if (!ok)  // loads in flight land before the CTA's memory goes
+          for (int n = max(0, kKParts * t + j - kKSlots); n < kKParts * t + j; ++n)
+            mbar_wait_drain(bar(kKFull0 + n % kKSlots), (uint32_t)(n / kKSlots) & 1u);
       }
-      if (!ok)  // loads in flight land before the CTA's memory goes
-        for (int k = max(0, n - kKSlots); k < n && k < total; ++k)
-          mbar_wait_drain(bar(kKFull0 + k % kKSlots), (uint32_t)(k / kKSlots) & 1u);
+      __syncwarp();
     } else if (warp == 1) {
       // ---- QK issuer: S buffer g % 3 <- Q . K^T, block by block ----
       const uint32_t idesc = idesc_bf16(128, 64, false, false);
       ok = wait_warp(bar(kQFull), 0u, abort_flag);
       tc_fence_after();
-      int n = 0;
       for (int g = 0; g < ntiles && ok; ++g) {
         const uint32_t b = (uint32_t)g % kSBufs;
         if (g >= kSBufs && !(ok = wait_warp(bar(kSFree0 + b), (uint32_t)(g / kSBufs - 1) & 1u, abort_flag))) break;
         const uint32_t d = tmem + kTmemS + b * 64u;
-        for (int j = 0; j < 9; ++j, ++n) {
-          const uint32_t s = (uint32_t)n % kKSlots;
-          if (!(ok = wait_warp(bar(kKFull0 + s), (uint32_t)(n / kKSlots) & 1u, abort_flag))) break;
+        const uint32_t s0 = (uint32_t)(g & 1) * kKParts;
+        const uint64_t bd = smem_desc(base + kOffData + (uint32_t)(g & 1) * kKTile, 16, 1024, kLayoutSw128);
+#pragma unroll
+        for (int part = 0; part < kKParts; ++part) {
+          if (!(ok = wait_warp(bar(kKFull0 + s0 + part), (uint32_t)(g >> 1) & 1u, abort_flag))) break;
           tc_fence_after();
-          const uint32_t slot = base + kOffData + s * kBlk;
           if (elect_one()) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              mma_bf16_ts(d, tmem + kTmemQ + (uint32_t)(j * 4 + k) * 8u,
-                          smem_desc(slot + (uint32_t)k * 32u, 16, 1024, kLayoutSw128), idesc, (j | k) ? 1u : 0u);
-            mma_commit(bar(kKFree0 + s));
-            if (j == 8) mma_commit(bar(kSFull0 + b));
+            for (int j = 4 * part; j < (part < 2 ? 4 * part + 4 : 9); ++j)
+#pragma unroll
+              for (int k = 0; k < 4; ++k)  // offsets in the descriptor's 16-byte units; 16 dims are 32 bytes
+                mma_bf16_ts(d, tmem + kTmemQ + (uint32_t)(j * 4 + k) * 8u, bd + (uint64_t)(j * (kBlk / 16u) + 2 * k), idesc,
+                            (j | k) ? 1u : 0u);
+            mma_commit(bar(kKFree0 + s0 + part));
+            if (part == kKParts - 1) mma_commit(bar(kSFull0 + b));
           }
           __syncwarp();
         }
@@ -395,9 +396,13 @@ __global__ void __launch_bounds__(kPxThreads, 1) fwd_prefix_kernel(const PrefixP
         }
         l += (s0 + s1) + (s2 + s3);
         const uint32_t flag = __any_sync(0xffffffffu, resc) ? 1u : 0u;
-        // the staging slot's message of tile g - 2 has landed
-        if (g >= kLSlots && !(ok = wait_warp(bar(kLFree0 + e), (uint32_t)(g / kLSlots - 1) & 1u, abort_flag, true))) break;
-        uint8_t* const slot = sbase + kOffLocal + (uint32_t)e * kSlotBytes;
+        // the staging slot's message of tile g - 4 has landed: its PV is done
+        if (g >= kLSlots) {
+          const uint32_t gp = (uint32_t)(g - kLSlots);
+          if (!(ok = wait_warp(bar(kPDone0 + gp % kPSlots), (gp / kPSlots) & 1u, abort_flag))) break;
+        }
+        const uint32_t ls = (uint32_t)g % kLSlots;
+        uint8_t* const slot = sbase + kOffLocal + ls * kSlotBytes;
         uint8_t* const prow = slot + (uint32_t)(row >> 3) * 1024u + (uint32_t)(row & 7) * 128u;
 #pragma unroll
         for (int q = 0; q < 8; ++q)
@@ -407,7 +412,7 @@ __global__ void __launch_bounds__(kPxThreads, 1) fwd_prefix_kernel(const PrefixP
         if (lane == 0) *reinterpret_cast<uint32_t*>(slot + kFlagOff + (uint32_t)quad * 4u) = flag;
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar(kLFull0 + e));
+        if (lane == 0) mbar_arrive(bar(kLFull0 + ls));
       }
       // ---- totals of the two groups ----
       if (ok) {
@@ -440,34 +445,30 @@ __global__ void __launch_bounds__(kPxThreads, 1) fwd_prefix_kernel(const PrefixP
   } else {
     // =============================== value CTA ===============================
     if (warp == 0) {
-      // ---- TMA: half tile n = 2 t + h into slot n % kVSlots ----
-      int n = 0;
-      for (; n < 2 * ntiles; ++n) {
-        const uint32_t s = (uint32_t)n % kVSlots;
-        if (n >= kVSlots && !(ok = wait_warp(bar(kVFree0 + s), (uint32_t)(n / kVSlots - 1) & 1u, abort_flag))) break;
-        if (elect_one()) {
+      // ---- TMA: half tile n = 2 t + h into slot n % kVSlots; one thread ----
+      if (lane == 0) {
+        int n = 0;
+        for (; n < 2 * ntiles; ++n) {
+          const uint32_t s = (uint32_t)n % kVSlots;
+          if (n >= kVSlots && !(ok = mbar_wait(bar(kVFree0 + s), (uint32_t)(n / kVSlots - 1) & 1u, abort_flag))) break;
           mbar_arrive_expect_tx(bar(kVFull0 + s), kHalf);
-          tma_load_3d(base + kOffData + s * kHalf, &maps.v, (tile0 + (n >> 1)) * 64, (n & 1) * 4, bar(kVFull0 + s));
+          tma_load_3d(base + kOffData + s * kHalf, &maps.half, (tile0 + (n >> 1)) * 64, (n & 1) * 4, bar(kVFull0 + s));
         }
-        __syncwarp();
+        if (!ok)
+          for (int k = max(0, n - kVSlots); k < n; ++k)
+            mbar_wait_drain(bar(kVFull0 + k % kVSlots), (uint32_t)(k / kVSlots) & 1u);
       }
-      if (!ok)
-        for (int k = max(0, n - kVSlots); k < n; ++k)
-          mbar_wait_drain(bar(kVFull0 + k % kVSlots), (uint32_t)(k / kVSlots) & 1u);
+      __syncwarp();
     } else if (warp == 1) {
       // ---- PV issuer ----
       const uint32_t idesc = idesc_bf16(128, 256, false, true);
       volatile uint32_t* const req = reinterpret_cast<volatile uint32_t*>(sbase + kOffReq);
-      const uint32_t r_lfree0 = mapa_shared(bar(kLFree0), 0);
       uint32_t nresc = 0;
       for (int g = 0; g < ntiles && ok; ++g) {
         const uint32_t s = (uint32_t)g % kPSlots;
         if (!(ok = wait_warp(bar(kPFull0 + s), (uint32_t)(g / kPSlots) & 1u, abort_flag, true))) break;
         const uint32_t slot = base + kOffSlot + s * kSlotBytes;
-        if (elect_one()) {
-          mbar_arrive_remote(r_lfree0 + 8u * ((uint32_t)g % kLSlots));          // the staging slot may be written again
-          if (g + kPSlots < ntiles) mbar_arrive_expect_tx(bar(kPFull0 + s), kMsgBytes);  // its next message
-        }
+        if (lane == 0 && g + kPSlots < ntiles) mbar_arrive_expect_tx(bar(kPFull0 + s), kMsgBytes);  // its next message
         __syncwarp();
         const volatile uint32_t* fl = reinterpret_cast<const volatile uint32_t*>(sbase + (slot - base) + kFlagOff);
         if ((fl[0] | fl[1] | fl[2] | fl[3]) != 0u) {
@@ -720,7 +721,7 @@ int prefix_max_clusters() {
 
 cudaError_t launch_fwd_prefix(const PrefixParams& p, const void* kv, const void* k_rope, cudaStream_t stream) {
   Maps maps;
-  if (!encode(&maps.k, kv, p.keys, 8, 1) || !encode(&maps.v, kv, p.keys, 8, 4) || !encode(&maps.rope, k_rope, p.keys, 1, 1))
+  if (!encode(&maps.half, kv, p.keys, 8, 4) || !encode(&maps.rope, k_rope, p.keys, 1, 1))
     return cudaErrorInvalidValue;
   const long long items = (p.rows + kPxRows - 1) / kPxRows * p.split;
   if (items <= 0 || 2 * items > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
