@@ -16,8 +16,8 @@
 //
 // Keys come by TMA (one 3-D map that turns a row of 512 into eight 64-wide
 // blocks, 128-byte swizzle) in half tiles of 64 keys x 256 dims (32 KB), each
-// released by the MMAs that read it: a ring of 5 in the value CTA, two tiles
-// of two halves and a rope block in the score CTA. A box costs its issuer some
+// released by the MMAs that read it: two tiles of two halves in either CTA, and
+// a rope block per tile in the score CTA. A box costs its issuer some
 // 300 cycles whatever its size, so 8 KB boxes cannot keep a tile's pace (nine
 // of them 3,200 cycles), and 32 KB ones can; whole tiles would keep fewer
 // bytes in flight.
@@ -25,9 +25,10 @@
 // P rounds the weights to BF16 for the MMA; the row sum adds them before the
 // rounding, in FP32 (as every other family here).
 //
-// Roles (12 warps): score CTA 0 TMA, 1 QK issuer, 2 P sender, 4-11 softmax
-// (warps 4-7 the even, 8-11 the odd tiles; the running maximum goes from one
-// to the other); value CTA 0 TMA, 1 PV issuer, 4-11 rescale and epilogue.
+// Roles (12 warps): score CTA 0 TMA, 1 and 3 QK issuers of the even and the
+// odd tiles, 2 P sender, 4-11 softmax (warps 4-7 the even, 8-11 the odd tiles;
+// the running maximum goes from one to the other); value CTA 0 TMA, 1 and 3 PV
+// issuers of the lower and the upper 256 columns, 4-11 rescale and epilogue.
 // Every wait is bounded and reports through the status word. No multicast
 // loads.
 #include <cuda.h>
@@ -47,9 +48,9 @@ constexpr uint32_t kHalf = 4u * kBlk;        // 64 keys x 256 value columns
 constexpr int kKParts = 3;                   // score CTA: dims 0-255, 256-511 and rope of a tile
 constexpr int kKSlots = 2 * kKParts;         // two tiles
 constexpr uint32_t kKTile = 2u * kHalf + kBlk;
-constexpr int kVSlots = 5;                   // value CTA: ring of V half tiles
-constexpr int kSBufs = 3;
-constexpr int kPSlots = 3;                   // value CTA
+constexpr int kVSlots = 4;                   // value CTA: ring of V half tiles, two tiles
+constexpr int kSBufs = 2;                    // S buffer g % 2: QK issuer g % 2 fills it, softmax group g % 2 reads it
+constexpr int kPSlots = 4;                   // value CTA
 constexpr int kLSlots = 4;                   // score CTA: P staging (even: slot g % 4 is softmax group g % 2's)
 constexpr uint32_t kPBytes = 128u * 64u * 2u;
 constexpr uint32_t kAlphaOff = kPBytes;
@@ -76,8 +77,8 @@ enum Bar {
   kReq = kPFull0 + kPSlots,         // a rescale request is posted
   kReqDone,
   kFin,                             // (l, f) landed
-  kDrain,                           // abort path: issued MMAs are done
-  kBarCount
+  kDrain0,                          // 2: abort path, an issuer's MMAs are done
+  kBarCount = kDrain0 + 2
 };
 constexpr uint32_t kOffTmemSlot = kBarCount * 8u;
 constexpr uint32_t kOffAbort = kOffTmemSlot + 8u;
@@ -220,8 +221,8 @@ __global__ void __launch_bounds__(kPxThreads, 1) fwd_prefix_kernel(const PrefixP
       mbar_init(bar(kReqDone), kEpiWarps);
       mbar_init(bar(kFin), 1);
     }
-    for (int s = 0; s < kPSlots; ++s) mbar_init(bar(kPDone0 + s), 1);
-    mbar_init(bar(kDrain), 1);
+    for (int s = 0; s < kPSlots; ++s) mbar_init(bar(kPDone0 + s), 2);  // both halves of the columns
+    for (int i = 0; i < 2; ++i) mbar_init(bar(kDrain0 + i), 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -261,17 +262,18 @@ __global__ void __launch_bounds__(kPxThreads, 1) fwd_prefix_kernel(const PrefixP
             mbar_wait_drain(bar(kKFull0 + n % kKSlots), (uint32_t)(n / kKSlots) & 1u);
       }
       __syncwarp();
-    } else if (warp == 1) {
-      // ---- QK issuer: S buffer g % 3 <- Q . K^T, block by block ----
+    } else if (warp == 1 || warp == 3) {
+      // ---- QK issuer i: S buffer i <- Q . K^T for tiles g = i mod 2, part by part (an issuer is held while
+      // its MMAs run; the other one's waits fall into that time) ----
+      const int i = warp >> 1;
       const uint32_t idesc = idesc_bf16(128, 64, false, false);
       ok = wait_warp(bar(kQFull), 0u, abort_flag);
       tc_fence_after();
-      for (int g = 0; g < ntiles && ok; ++g) {
-        const uint32_t b = (uint32_t)g % kSBufs;
-        if (g >= kSBufs && !(ok = wait_warp(bar(kSFree0 + b), (uint32_t)(g / kSBufs - 1) & 1u, abort_flag))) break;
-        const uint32_t d = tmem + kTmemS + b * 64u;
-        const uint32_t s0 = (uint32_t)(g & 1) * kKParts;
-        const uint64_t bd = smem_desc(base + kOffData + (uint32_t)(g & 1) * kKTile, 16, 1024, kLayoutSw128);
+      const uint32_t d = tmem + kTmemS + (uint32_t)i * 64u;
+      const uint32_t s0 = (uint32_t)(i * kKParts);
+      const uint64_t bd = smem_desc(base + kOffData + (uint32_t)i * kKTile, 16, 1024, kLayoutSw128);
+      for (int g = i; g < ntiles && ok; g += 2) {
+        if (g >= 2 && !(ok = wait_warp(bar(kSFree0 + i), (uint32_t)((g >> 1) - 1) & 1u, abort_flag))) break;
 #pragma unroll
         for (int part = 0; part < kKParts; ++part) {
           if (!(ok = wait_warp(bar(kKFull0 + s0 + part), (uint32_t)(g >> 1) & 1u, abort_flag))) break;
@@ -284,18 +286,18 @@ __global__ void __launch_bounds__(kPxThreads, 1) fwd_prefix_kernel(const PrefixP
                 mma_bf16_ts(d, tmem + kTmemQ + (uint32_t)(j * 4 + k) * 8u, bd + (uint64_t)(j * (kBlk / 16u) + 2 * k), idesc,
                             (j | k) ? 1u : 0u);
             mma_commit(bar(kKFree0 + s0 + part));
-            if (part == kKParts - 1) mma_commit(bar(kSFull0 + b));
+            if (part == kKParts - 1) mma_commit(bar(kSFull0 + i));
           }
           __syncwarp();
         }
       }
       if (!ok) {
-        if (elect_one()) mma_commit(bar(kDrain));
+        if (elect_one()) mma_commit(bar(kDrain0 + i));
         __syncwarp();
-        mbar_wait_drain(bar(kDrain), 0u);
+        mbar_wait_drain(bar(kDrain0 + i), 0u);
       }
     } else if (warp == 2) {
-      // ---- P sender: staging slot g % 2 -> the value CTA's P slot g % 3 ----
+      // ---- P sender: staging slot g % 4 -> the value CTA's P slot g % 4 ----
       const uint32_t r_slot0 = mapa_shared(base + kOffSlot, 1);
       const uint32_t r_pfull0 = mapa_shared(bar(kPFull0), 1);
       int g = 0;
@@ -459,8 +461,9 @@ __global__ void __launch_bounds__(kPxThreads, 1) fwd_prefix_kernel(const PrefixP
             mbar_wait_drain(bar(kVFull0 + k % kVSlots), (uint32_t)(k / kVSlots) & 1u);
       }
       __syncwarp();
-    } else if (warp == 1) {
-      // ---- PV issuer ----
+    } else if (warp == 1 || warp == 3) {
+      // ---- PV issuer h: O[:, 256 h .. 256 h + 255] += P . V; issuer 0 posts the requests ----
+      const int h = warp >> 1;
       const uint32_t idesc = idesc_bf16(128, 256, false, true);
       volatile uint32_t* const req = reinterpret_cast<volatile uint32_t*>(sbase + kOffReq);
       uint32_t nresc = 0;
@@ -468,11 +471,11 @@ __global__ void __launch_bounds__(kPxThreads, 1) fwd_prefix_kernel(const PrefixP
         const uint32_t s = (uint32_t)g % kPSlots;
         if (!(ok = wait_warp(bar(kPFull0 + s), (uint32_t)(g / kPSlots) & 1u, abort_flag, true))) break;
         const uint32_t slot = base + kOffSlot + s * kSlotBytes;
-        if (lane == 0 && g + kPSlots < ntiles) mbar_arrive_expect_tx(bar(kPFull0 + s), kMsgBytes);  // its next message
+        if (h == 0 && lane == 0 && g + kPSlots < ntiles) mbar_arrive_expect_tx(bar(kPFull0 + s), kMsgBytes);  // its next message
         __syncwarp();
         const volatile uint32_t* fl = reinterpret_cast<const volatile uint32_t*>(sbase + (slot - base) + kFlagOff);
         if ((fl[0] | fl[1] | fl[2] | fl[3]) != 0u) {
-          if (elect_one()) {
+          if (h == 0 && lane == 0) {
             *req = (uint32_t)g;
             mbar_arrive(bar(kReq));
           }
@@ -481,44 +484,40 @@ __global__ void __launch_bounds__(kPxThreads, 1) fwd_prefix_kernel(const PrefixP
           ++nresc;
         }
         const int valid = used - (tile0 + g) * 64;
-#pragma unroll 1
-        for (int h = 0; h < 2; ++h) {
-          const int n = 2 * g + h;
-          const uint32_t vs = (uint32_t)n % kVSlots;
-          if (!(ok = wait_warp(bar(kVFull0 + vs), (uint32_t)(n / kVSlots) & 1u, abort_flag))) break;
-          const uint32_t vslot = base + kOffData + vs * kHalf;
-          if (valid < 64) {
-            // rows behind the last key: weight 0, but 0 x NaN of a cache row never written would not be 0
-            for (int i = lane; i < (64 - valid) * 32; i += 32) {
-              const int r = valid + (i >> 5), q = i & 31;
-              *reinterpret_cast<uint4*>(sbase + (vslot - base) + (uint32_t)(q >> 3) * kBlk + (uint32_t)r * 128u +
-                                        (uint32_t)(q & 7) * 16u) = make_uint4(0, 0, 0, 0);
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
+        const uint32_t vs = (uint32_t)(2 * g + h) % kVSlots;
+        if (!(ok = wait_warp(bar(kVFull0 + vs), (uint32_t)(g >> 1) & 1u, abort_flag))) break;
+        const uint32_t vslot = base + kOffData + vs * kHalf;
+        if (valid < 64) {
+          // rows behind the last key: weight 0, but 0 x NaN of a cache row never written would not be 0
+          for (int i = lane; i < (64 - valid) * 32; i += 32) {
+            const int r = valid + (i >> 5), q = i & 31;
+            *reinterpret_cast<uint4*>(sbase + (vslot - base) + (uint32_t)(q >> 3) * kBlk + (uint32_t)r * 128u +
+                                      (uint32_t)(q & 7) * 16u) = make_uint4(0, 0, 0, 0);
           }
-          tc_fence_after();
-          if (elect_one()) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              mma_bf16_ss(tmem + kTmemO + h * 256, smem_desc(slot + j * 32, 16, 1024, kLayoutSw128),
-                          smem_desc(vslot + j * 2048, kBlk, 1024, kLayoutSw128), idesc, (g | j) ? 1u : 0u);
-            mma_commit(bar(kVFree0 + vs));
-            if (h == 1) mma_commit_mc(bar(kPDone0 + s), (uint16_t)3);
-          }
+          fence_proxy_async_smem();
           __syncwarp();
         }
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            mma_bf16_ss(tmem + kTmemO + h * 256, smem_desc(slot + j * 32, 16, 1024, kLayoutSw128),
+                        smem_desc(vslot + j * 2048, kBlk, 1024, kLayoutSw128), idesc, (g | j) ? 1u : 0u);
+          mma_commit(bar(kVFree0 + vs));
+          mma_commit_mc(bar(kPDone0 + s), (uint16_t)3);
+        }
+        __syncwarp();
       }
       if (ok) {
-        if (elect_one()) {
+        if (h == 0 && lane == 0) {
           *req = kReqEnd;
           mbar_arrive(bar(kReq));
         }
         __syncwarp();
       } else {
-        if (elect_one()) mma_commit(bar(kDrain));
+        if (elect_one()) mma_commit(bar(kDrain0 + h));
         __syncwarp();
-        mbar_wait_drain(bar(kDrain), 0u);
+        mbar_wait_drain(bar(kDrain0 + h), 0u);
       }
     } else if (warp >= kSoftWarp0) {
       // ---- rescale requests, then the epilogue: half `part` of the columns of 32 rows ----
