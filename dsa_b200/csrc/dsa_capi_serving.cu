@@ -75,11 +75,13 @@ bool plan_prefix(const dsa_fwd_args_t* a, const dsa_prefix_kv_t* px, PrefixPlan*
   plan->own_split = 0;
   if (own) {
     // own keys: one wave of the pair (H = 128) or stream family's CTAs, two
-    // tiles of 32 keys at least per split
+    // tiles of 32 keys at least per split; items of at most 64 tiles, which
+    // fill the SMs that the prefix leaves or frees
     const int64_t tiles = (a->topk + 31) / 32;
     int64_t ctas = a->heads == 128 ? dsa::pair_max_ctas() / 2 : dsa::stream_max_ctas();
     if (ctas <= 0) ctas = a->heads == 128 ? 74 : 296;
     int64_t s = ctas / (a->heads == 128 ? plan->tokens : plan->tokens * (a->heads / 16));
+    if (s < (tiles + 63) / 64) s = (tiles + 63) / 64;
     if (s > tiles / 2) s = tiles / 2;
     if (s > 16) s = 16;
     plan->own_split = (int)(s < 1 ? 1 : s);
@@ -291,6 +293,7 @@ int dsa_sparse_mla_fwd_prefix(const dsa_fwd_args_t* a, const dsa_prefix_kv_t* px
     f.split = plan.own_split;
     f.keys_per_tile = 32;
     f.heads_per_cta = a->heads == 128 ? 128 : 16;
+    f.beside_previous = 1;  // fills the SMs that the prefix kernel leaves
     st = launch_status(a->heads == 128 ? dsa::launch_fwd_pair(f, s) : dsa::launch_fwd_stream(f, s, false));
     if (st != DSA_STATUS_OK) return st;
   }

@@ -75,6 +75,10 @@ struct FwdParams {
   // barrier nothing arrives at, so the bound runs out (failure-path test).
   unsigned long long wait_limit_ns;
   int wait_test;
+  // The launch may run beside the kernel before it in the stream, on which
+  // nothing here depends, one item per cluster or CTA; it ends after that
+  // kernel, for which its last CTAs wait (pair and stream families).
+  int beside_previous;
 };
 
 // Host: fill scale_div / scale_log2 from the ABI's scale (0 = the
@@ -168,6 +172,12 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
   __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&v);
 }
+
+// Programmatic launches (no effect in a launch without them): let the stream's
+// next kernel start before this one ends; wait until the kernel before this
+// one has ended and its writes are visible.
+__device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 __device__ __forceinline__ void report_error(int32_t* status, int bits) {
   if (status != nullptr) atomicOr(status, bits);

@@ -942,16 +942,13 @@ __global__ void __launch_bounds__(kPrThreads, 1) fwd_pair_kernel(const FwdParams
         } else {
           const size_t pr = ((size_t)w.token * p.split + w.sp) * kPrHeads + row;
           float* dst = p.part_num + pr * kDimLatent;
+          const bool wide = (reinterpret_cast<uintptr_t>(p.part_num) & 31u) == 0;
 #pragma unroll 1
           for (int cb = cb0; cb < cb1; cb += 32) {
             uint32_t o[32];
             tmem_ld32(tmem + t_lane + kTmemO + cb, o);
             tmem_wait_ld();
-            float4* d4 = reinterpret_cast<float4*>(dst + cb);
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-              d4[k] = make_float4(u2f(o[4 * k]) * lf.y, u2f(o[4 * k + 1]) * lf.y, u2f(o[4 * k + 2]) * lf.y,
-                                  u2f(o[4 * k + 3]) * lf.y);
+            store_f32_row32(dst + cb, o, lf.y, wide);
           }
         }
         tc_fence_before();
@@ -961,6 +958,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) fwd_pair_kernel(const FwdParams
     }
   }
   if (!ok && lane == 0) report_error(p.status, kErrTimeout);
+  if (p.beside_previous && cid == ncl - 1) grid_dependency_wait();
 
   __syncwarp();
   tc_fence_before();
@@ -971,11 +969,14 @@ __global__ void __launch_bounds__(kPrThreads, 1) fwd_pair_kernel(const FwdParams
   }
 }
 
+// attr: two entries, the second used when cfg->numAttrs is raised to 2.
 bool pair_launch_config(cudaLaunchConfig_t* cfg, cudaLaunchAttribute* attr, int ctas, cudaStream_t stream) {
-  attr->id = cudaLaunchAttributeClusterDimension;
-  attr->val.clusterDim.x = 2;
-  attr->val.clusterDim.y = 1;
-  attr->val.clusterDim.z = 1;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   *cfg = cudaLaunchConfig_t{};
   cfg->gridDim = dim3((unsigned)ctas, 1, 1);
   cfg->blockDim = dim3(kPrThreads, 1, 1);
@@ -998,12 +999,12 @@ int pair_max_ctas() {
           cudaSuccess)
     return -1;
   cudaLaunchConfig_t cfg;
-  cudaLaunchAttribute attr;
+  cudaLaunchAttribute attr[2];
   int dev = 0, sms = 0;
   if (cudaGetDevice(&dev) != cudaSuccess ||
       cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0)
     return -1;
-  pair_launch_config(&cfg, &attr, sms & ~1, nullptr);
+  pair_launch_config(&cfg, attr, sms & ~1, nullptr);
   int clusters = 0;
   if (cudaOccupancyMaxActiveClusters(&clusters, fwd_pair_kernel<false>, &cfg) != cudaSuccess || clusters <= 0)
     return -1;
@@ -1016,10 +1017,13 @@ cudaError_t launch_fwd_pair(const FwdParams& p, cudaStream_t stream) {
   const int max_ctas = pair_max_ctas();
   if (max_ctas <= 0) return cudaErrorInvalidConfiguration;
   const long long items = (long long)p.tokens * p.split;
-  const long long clusters = items < max_ctas / 2 ? items : max_ctas / 2;
+  // beside another kernel: a cluster per item, which start as SMs become free
+  const long long clusters = p.beside_previous || items < max_ctas / 2 ? items : max_ctas / 2;
+  if (2 * clusters > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
   cudaLaunchConfig_t cfg;
-  cudaLaunchAttribute attr;
-  pair_launch_config(&cfg, &attr, (int)(2 * clusters), stream);
+  cudaLaunchAttribute attr[2];
+  pair_launch_config(&cfg, attr, (int)(2 * clusters), stream);
+  if (p.beside_previous) cfg.numAttrs = 2;
   return cudaLaunchKernelEx(&cfg, fwd_pair_kernel<false>, p);
 }
 
@@ -1034,8 +1038,8 @@ cudaError_t launch_fwd_pair_union(const FwdParams& p, cudaStream_t stream) {
   const long long items = p.tokens;
   const long long clusters = items < max_ctas / 2 ? items : max_ctas / 2;
   cudaLaunchConfig_t cfg;
-  cudaLaunchAttribute attr;
-  pair_launch_config(&cfg, &attr, (int)(2 * clusters), stream);
+  cudaLaunchAttribute attr[2];
+  pair_launch_config(&cfg, attr, (int)(2 * clusters), stream);
   return cudaLaunchKernelEx(&cfg, fwd_pair_kernel<true>, p);
 }
 

@@ -80,6 +80,15 @@ enum Bar {
   kDrain0,                          // 2: abort path, an issuer's MMAs are done
   kBarCount = kDrain0 + 2
 };
+// Arrivals that complete a phase.
+__device__ __forceinline__ uint32_t bar_count(int i) {
+  if (i == kQFull || i == kReqDone) return 8;                                  // softmax warps; epilogue warps
+  if (i >= kSFree0 && i < kSFree0 + kSBufs) return 4;                          // the group's warps
+  if (i >= kLFull0 && i < kLFull0 + kLSlots) return 4;
+  if (i >= kXchg0 && i < kXchg0 + 4) return 2;                                 // both groups' warps of the quadrant
+  if (i >= kPDone0 && i < kPDone0 + kPSlots) return 2;                         // both halves of the columns
+  return 1;
+}
 constexpr uint32_t kOffTmemSlot = kBarCount * 8u;
 constexpr uint32_t kOffAbort = kOffTmemSlot + 8u;
 constexpr uint32_t kOffReq = kOffAbort + 8u;
@@ -92,10 +101,18 @@ constexpr uint32_t kOffSlot = kOffData + kVSlots * kHalf;          // value CTA
 constexpr uint32_t kOffFin = kOffSlot + kPSlots * kSlotBytes;
 constexpr uint32_t kValueBytes = kOffFin + kFinBytes;
 constexpr uint32_t kSmemBytes = (kScoreBytes > kValueBytes ? kScoreBytes : kValueBytes) + 1024u;
+// The MMA cuts each of a score's 36 accumulations to FP32 instead of rounding
+// it: half a unit in the last place is lost on average, 2^-25 to 2^-24 of a sum
+// that has grown half way, together 36 / 2 * 2^-24.8 = 6e-7 of the score (5.6e-7
+// measured, always towards zero). Scaling by 1 + 5.6e-7 takes the mean error of
+// softmax_max from -5.6e-7 to below 1e-7 relative and with it that of softmax_sum,
+// which is relative to the maximum, from 1.8e-6 to 5e-7.
+constexpr double kCutBias = 5.6e-7;
 constexpr uint32_t kReqEnd = 0xffffffffu;
 constexpr uint32_t kTmemCols = 512, kTmemQ = 0, kTmemS = 288, kTmemO = 0;
 
-static_assert(kOffReq + 8u <= kOffData, "barrier block");
+static_assert(kOffReq + 8u <= kOffData && kBarCount <= kPxThreads, "barrier block");
+static_assert(kEpiWarps == 8, "bar_count");
 static_assert(kOffLocal % 1024 == 0 && kOffSlot % 1024 == 0 && kSlotBytes % 1024 == 0, "swizzle atoms");
 static_assert(kSmemBytes <= 232448, "shared memory budget");
 static_assert(kTmemS + kSBufs * 64 <= kTmemCols, "score TMEM budget");
@@ -141,21 +158,49 @@ struct Maps {
   CUtensorMap rope;  // rope, boxes of 64 keys x 64 dims
 };
 
-// Chunk `ch` (dims 64ch..; 8: rope) of one Q row -> 32 TMEM columns of this lane.
-__device__ __forceinline__ void load_q_chunk(const PrefixParams& p, size_t row, int ch, uint32_t taddr) {
-  const uint4* s4 = ch < 8 ? reinterpret_cast<const uint4*>(p.q + row * kDimLatent) + ch * 8
-                           : reinterpret_cast<const uint4*>(p.q_rope + row * kDimRope);
-  uint32_t r[32];
+// Chunks [c0, c0 + N) (dims 64c..; chunk 8: rope) of the 32 Q rows of this
+// warp -> TMEM, lane = row, 32 columns a chunk. The loads take whole 128-byte
+// lines, four rows an instruction (a lane reading its own row costs 32 line
+// lookups an instruction: 8,900 cycles for Q against 2,500), all chunks in flight
+// together; each goes through 4 KB of shared memory (swizzled) to become rows.
+template <int N>
+__device__ __forceinline__ void load_q_chunks(const PrefixParams& p, long long row0, int lane, int c0, uint4 (*v)[8]) {
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const uint4 v = __ldg(s4 + k);
-    r[4 * k] = v.x;
-    r[4 * k + 1] = v.y;
-    r[4 * k + 2] = v.z;
-    r[4 * k + 3] = v.w;
-  }
-  tmem_st32(taddr, r);
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const size_t row = (size_t)min(row0 + 4 * k + (lane >> 3), p.rows - 1);  // rows past the end repeat the last one
+      v[i][k] = __ldg((c0 + i < 8 ? reinterpret_cast<const uint4*>(p.q + row * kDimLatent) + (c0 + i) * 8
+                                  : reinterpret_cast<const uint4*>(p.q_rope + row * kDimRope)) + (lane & 7));
+    }
 }
+template <int N>
+__device__ __forceinline__ void store_q_chunks(int lane, int c0, const uint4 (*v)[8], uint8_t* scratch, uint32_t tq) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int r = 4 * k + (lane >> 3);
+      *reinterpret_cast<uint4*>(scratch + r * 128 + (((lane & 7) ^ (r & 7)) * 16)) = v[i][k];
+    }
+    __syncwarp();
+    uint32_t out[32];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const uint4 w = *reinterpret_cast<const uint4*>(scratch + lane * 128 + ((k ^ (lane & 7)) * 16));
+      out[4 * k] = w.x;
+      out[4 * k + 1] = w.y;
+      out[4 * k + 2] = w.z;
+      out[4 * k + 3] = w.w;
+    }
+    tmem_st32(tq + (uint32_t)(c0 + i) * 32u, out);
+    __syncwarp();
+  }
+}
+
+// Split cluster barrier: what this thread wrote before the arrive is visible
+// to the peer's threads after their wait.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 
 __global__ void __launch_bounds__(kPxThreads, 1) fwd_prefix_kernel(const PrefixParams p,
                                                                    const __grid_constant__ Maps maps) {
@@ -169,6 +214,7 @@ __global__ void __launch_bounds__(kPxThreads, 1) fwd_prefix_kernel(const PrefixP
   const int mt = item / p.split, sp = item - mt * p.split;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(sbase + kOffAbort);
   auto bar = [&](int i) -> uint32_t { return base + 8u * (uint32_t)i; };
+  grid_launch_dependents();  // the own keys' kernel needs nothing from this one
 
   // keys [tile0 * 64, ...) of the split: whole tiles of the keys in use
   const int used = p.length != nullptr ? min(max(__ldg(p.length), 0), p.keys) : p.keys;
@@ -195,37 +241,14 @@ __global__ void __launch_bounds__(kPxThreads, 1) fwd_prefix_kernel(const PrefixP
     return;
   }
 
-  if (threadIdx.x == 0) {
-    if (rank == 0) {
-      for (int s = 0; s < kKSlots; ++s) {
-        mbar_init(bar(kKFull0 + s), 1);
-        mbar_init(bar(kKFree0 + s), 1);
-      }
-      mbar_init(bar(kQFull), 8);
-      for (int i = 0; i < kSBufs; ++i) {
-        mbar_init(bar(kSFull0 + i), 1);
-        mbar_init(bar(kSFree0 + i), 4);
-      }
-      for (int q = 0; q < 4; ++q) {
-        mbar_init(bar(kMReady0 + q), 1);
-        mbar_init(bar(kXchg0 + q), 2);
-      }
-      for (int s = 0; s < kLSlots; ++s) mbar_init(bar(kLFull0 + s), 4);
-    } else {
-      for (int s = 0; s < kVSlots; ++s) {
-        mbar_init(bar(kVFull0 + s), 1);
-        mbar_init(bar(kVFree0 + s), 1);
-      }
-      for (int s = 0; s < kPSlots; ++s) mbar_init(bar(kPFull0 + s), 1);
-      mbar_init(bar(kReq), 1);
-      mbar_init(bar(kReqDone), kEpiWarps);
-      mbar_init(bar(kFin), 1);
-    }
-    for (int s = 0; s < kPSlots; ++s) mbar_init(bar(kPDone0 + s), 2);  // both halves of the columns
-    for (int i = 0; i < 2; ++i) mbar_init(bar(kDrain0 + i), 1);
-    *abort_flag = 0;
-    fence_barrier_init();
-  }
+  // the softmax warps' first two chunks of Q are under way while the CTA sets up
+  uint4 q_first[3][8];
+  if (rank == 0 && warp >= kSoftWarp0)
+    load_q_chunks<2>(p, row0 + (warp & 3) * 32, lane, 5 * ((warp - kSoftWarp0) >> 2), q_first);
+  // one barrier per thread (each CTA uses its own part of them)
+  if (threadIdx.x < kBarCount) mbar_init(bar((int)threadIdx.x), bar_count((int)threadIdx.x));
+  if (threadIdx.x == 0) *abort_flag = 0;
+  fence_barrier_init();
   if (warp == 0) {
     tmem_alloc(base + kOffTmemSlot, kTmemCols);
     tmem_relinquish();
@@ -238,7 +261,10 @@ __global__ void __launch_bounds__(kPxThreads, 1) fwd_prefix_kernel(const PrefixP
     for (int s = 0; s < kPSlots; ++s) mbar_arrive_expect_tx(bar(kPFull0 + s), kMsgBytes);
     mbar_arrive_expect_tx(bar(kFin), kFinBytes);
   }
-  cluster_sync();
+  __syncwarp();
+  // Each role waits for the peer CTA's barriers before it first addresses the
+  // peer, or at its end; loads and Q start without it.
+  cluster_arrive();
 
   bool ok = true;
   if (rank == 0) {
@@ -262,6 +288,7 @@ __global__ void __launch_bounds__(kPxThreads, 1) fwd_prefix_kernel(const PrefixP
             mbar_wait_drain(bar(kKFull0 + n % kKSlots), (uint32_t)(n / kKSlots) & 1u);
       }
       __syncwarp();
+      cluster_wait();
     } else if (warp == 1 || warp == 3) {
       // ---- QK issuer i: S buffer i <- Q . K^T for tiles g = i mod 2, part by part (an issuer is held while
       // its MMAs run; the other one's waits fall into that time) ----
@@ -296,10 +323,13 @@ __global__ void __launch_bounds__(kPxThreads, 1) fwd_prefix_kernel(const PrefixP
         __syncwarp();
         mbar_wait_drain(bar(kDrain0 + i), 0u);
       }
+      __syncwarp();
+      cluster_wait();
     } else if (warp == 2) {
       // ---- P sender: staging slot g % 4 -> the value CTA's P slot g % 4 ----
       const uint32_t r_slot0 = mapa_shared(base + kOffSlot, 1);
       const uint32_t r_pfull0 = mapa_shared(bar(kPFull0), 1);
+      cluster_wait();
       int g = 0;
       for (; g < ntiles; ++g) {
         const uint32_t ls = (uint32_t)g % kLSlots, ps = (uint32_t)g % kPSlots;
@@ -323,14 +353,22 @@ __global__ void __launch_bounds__(kPxThreads, 1) fwd_prefix_kernel(const PrefixP
       float* const mpub = reinterpret_cast<float*>(sbase + kOffM);
       float* const xch = reinterpret_cast<float*>(sbase + kOffX);
       {
-        const size_t qrow = (size_t)min(row0 + row, p.rows - 1);  // rows past the end repeat the last one
+        // scratch in the P staging slots: P of a tile is written after every warp's Q is loaded
+        uint8_t* const scratch = sbase + kOffLocal + (warp - kSoftWarp0) * 4096;
         const uint32_t tq = tmem + t_lane + kTmemQ;
-#pragma unroll 1
-        for (int ch = e * 5; ch < (e == 0 ? 5 : 9); ++ch) load_q_chunk(p, qrow, ch, tq + (uint32_t)ch * 32u);
+        store_q_chunks<2>(lane, 5 * e, q_first, scratch, tq);
+        if (e == 0) {
+          load_q_chunks<3>(p, row0 + quad * 32, lane, 2, q_first);
+          store_q_chunks<3>(lane, 2, q_first, scratch, tq);
+        } else {
+          load_q_chunks<2>(p, row0 + quad * 32, lane, 7, q_first);
+          store_q_chunks<2>(lane, 7, q_first, scratch, tq);
+        }
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(kQFull));
+        cluster_wait();
       }
       float m_w = kNegFltMax, m_true = kNegFltMax, l = 0.f;
       for (int g = e; g < ntiles; g += 2) {
@@ -461,9 +499,11 @@ __global__ void __launch_bounds__(kPxThreads, 1) fwd_prefix_kernel(const PrefixP
             mbar_wait_drain(bar(kVFull0 + k % kVSlots), (uint32_t)(k / kVSlots) & 1u);
       }
       __syncwarp();
+      cluster_wait();
     } else if (warp == 1 || warp == 3) {
       // ---- PV issuer h: O[:, 256 h .. 256 h + 255] += P . V; issuer 0 posts the requests ----
       const int h = warp >> 1;
+      cluster_wait();
       const uint32_t idesc = idesc_bf16(128, 256, false, true);
       volatile uint32_t* const req = reinterpret_cast<volatile uint32_t*>(sbase + kOffReq);
       uint32_t nresc = 0;
@@ -522,6 +562,7 @@ __global__ void __launch_bounds__(kPxThreads, 1) fwd_prefix_kernel(const PrefixP
     } else if (warp >= kSoftWarp0) {
       // ---- rescale requests, then the epilogue: half `part` of the columns of 32 rows ----
       const int quad = warp & 3, part = (warp - kSoftWarp0) >> 2;
+      cluster_wait();
       const int row = quad * 32 + lane;
       const uint32_t t_o = tmem + ((uint32_t)(quad * 32) << 16) + kTmemO + (uint32_t)part * 256u;
       const volatile uint32_t* const req = reinterpret_cast<const volatile uint32_t*>(sbase + kOffReq);
@@ -570,17 +611,27 @@ __global__ void __launch_bounds__(kPxThreads, 1) fwd_prefix_kernel(const PrefixP
             if (grow < p.rows) store_bf16_row32_paired(dst + cb, kDimLatent, a, b, wide);  // rows is even: pairs are whole
           }
         } else {
-          float* const dst = p.part_num + ((size_t)item * kPxRows + row) * kDimLatent + part * 256;
+          // [64 groups of 8 columns][128 rows][8]: a store instruction writes 1 KB in a row
+          float* const dst = p.part_num + ((size_t)item * 64 + part * 32) * (kPxRows * 8) + row * 8;
+          const bool live = grow < p.rows;
 #pragma unroll 1
-          for (int cb = 0; cb < 256; cb += 32) {
-            uint32_t o[32];
+          for (int cb = 0; cb < 256 && row0 + quad * 32 < p.rows; cb += 64) {
+            uint32_t o[64];
             tmem_ld32(t_o + (uint32_t)cb, o);
+            tmem_ld32(t_o + (uint32_t)cb + 32u, o + 32);
             tmem_wait_ld_regs32(o);
-            if (grow < p.rows) store_f32_row32(dst + cb, o, f, true);
+            tmem_wait_ld_regs32(o + 32);
+#pragma unroll
+            for (int k = 0; k < 64; ++k) o[k] = f2u(u2f(o[k]) * f);
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              if (live) st_global_v8(dst + (size_t)(cb / 8 + k) * (kPxRows * 8), o + 8 * k);
           }
         }
         tc_fence_before();
       }
+    } else {
+      cluster_wait();
     }
   }
   if (!ok && lane == 0) report_error(p.status, kErrTimeout);
@@ -594,61 +645,89 @@ __global__ void __launch_bounds__(kPxThreads, 1) fwd_prefix_kernel(const PrefixP
 }
 
 // Join of a row's prefix partials and its own-key partials: m = max m_i,
-// out = sum_i e^(m_i - m) n_i / sum_i e^(m_i - m) l_i. One warp per row, a
-// lane's columns are 4 lane + 128 k; parts with sum 0 are not read.
-__global__ void __launch_bounds__(256) prefix_join_kernel(const JoinParams p) {
-  const int lane = threadIdx.x & 31;
-  const long long r = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (r >= p.rows) return;
-  const long long mt = r >> 7;
+// out = sum_i e^(m_i - m) n_i / sum_i e^(m_i - m) l_i. A block takes 32 rows
+// (lane = row) and 64 columns (8 a warp); the weights of its rows' parts are
+// computed once in shared memory. Bound by the partials' 2 KB a row and part:
+// 32-byte loads, four parts in flight. A part of weight 0 is not read.
+constexpr int kJoinWarps = 8;
+constexpr int kJoinMaxParts = 160;
+
+__global__ void __launch_bounds__(32 * kJoinWarps) prefix_join_kernel(const JoinParams p) {
+  __shared__ float weight[kJoinMaxParts][32];
+  __shared__ float red[kJoinWarps][32];
+  grid_dependency_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long r = (long long)blockIdx.x * 32 + lane;
+  const bool live = r < p.rows;
+  const long long rr = live ? r : p.rows - 1;
   const int n = p.split + p.own_split;
-  const long long token = r / p.heads;
-  auto at = [&](int i, const float*& num, float& m, float& l) {
-    if (i < p.split) {
-      const size_t k = (size_t)(mt * p.split + i) * kPxRows + (size_t)(r & 127);
-      num = p.part_num + k * kDimLatent;
-      m = p.part_max[k];
-      l = p.part_sum[k];
-    } else {
-      const size_t k = ((size_t)token * p.own_split + (i - p.split)) * p.heads + (size_t)(r - token * p.heads);
-      num = p.own_num + k * kDimLatent;
-      m = p.own_max[k];
-      l = p.own_sum[k];
-    }
+  const long long token = rr / p.heads;
+  const long long px0 = (rr >> 7) * p.split;                                 // + part: [.., 128] rows
+  const long long own0 = token * p.own_split * p.heads + (rr - token * p.heads);  // + part * heads
+  auto stat = [&](int i) {
+    const bool px = i < p.split;
+    const long long k = px ? (px0 + i) * kPxRows + (rr & 127) : own0 + (long long)(i - p.split) * p.heads;
+    return px ? make_float2(p.part_max[k], p.part_sum[k]) : make_float2(p.own_max[k], p.own_sum[k]);
   };
   float top = kNegFltMax;
-  for (int i = 0; i < n; ++i) {
-    const float* num;
-    float m, l;
-    at(i, num, m, l);
-    if (l != 0.f) top = fmaxf(top, m);
+  for (int i = warp; i < n; i += kJoinWarps) {
+    const float2 ml = stat(i);
+    if (ml.y != 0.f) top = fmaxf(top, ml.x);
   }
-  float4 acc[4];
+  red[warp][lane] = top;
+  __syncthreads();
 #pragma unroll
-  for (int k = 0; k < 4; ++k) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k = 0; k < kJoinWarps; ++k) top = fmaxf(top, red[k][lane]);
+  __syncthreads();
+  float part = 0.f;
+  for (int i = warp; i < n; i += kJoinWarps) {
+    const float2 ml = stat(i);
+    const float w = ml.y != 0.f ? expf(ml.x - top) : 0.f;
+    weight[i][lane] = w;
+    part += w * ml.y;
+  }
+  red[warp][lane] = part;
+  __syncthreads();
   float total = 0.f;
-  for (int i = 0; i < n; ++i) {
-    const float* num;
-    float m, l;
-    at(i, num, m, l);
-    if (l == 0.f) continue;
-    const float w = expf(m - top);
-    total += w * l;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float4 v = *reinterpret_cast<const float4*>(num + 4 * lane + 128 * k);
-      acc[k].x = fmaf(w, v.x, acc[k].x);
-      acc[k].y = fmaf(w, v.y, acc[k].y);
-      acc[k].z = fmaf(w, v.z, acc[k].z);
-      acc[k].w = fmaf(w, v.w, acc[k].w);
+  for (int k = 0; k < kJoinWarps; ++k) total += red[k][lane];
+  const int col = blockIdx.y * (8 * kJoinWarps) + warp * 8;
+  const float* const px_src = p.part_num + ((size_t)px0 * 64 + col / 8) * (kPxRows * 8) + (rr & 127) * 8;
+  const float* const own_src = p.own_num + (size_t)own0 * kDimLatent + col;
+  float acc[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) acc[k] = 0.f;
+  for (int i0 = 0; i0 < n; i0 += 4) {
+    float4 v[4][2];
+    float w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int i = i0 + j;
+      w[j] = i < n ? weight[i][lane] : 0.f;
+      v[j][0] = v[j][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (w[j] != 0.f) {
+        const float* const src = i < p.split ? px_src + (size_t)i * (64 * kPxRows * 8)
+                                             : own_src + (size_t)(i - p.split) * p.heads * kDimLatent;
+        v[j][0] = reinterpret_cast<const float4*>(src)[0];
+        v[j][1] = reinterpret_cast<const float4*>(src)[1];
+      }
     }
-  }
-  const float rl = total != 0.f ? __frcp_rn(total) : 0.f;
 #pragma unroll
-  for (int k = 0; k < 4; ++k)
-    *reinterpret_cast<uint2*>(p.out + r * kDimLatent + 4 * lane + 128 * k) =
-        make_uint2(pack_bf16x2(acc[k].x * rl, acc[k].y * rl), pack_bf16x2(acc[k].z * rl, acc[k].w * rl));
-  if (lane == 0) {
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        acc[4 * h] = fmaf(w[j], v[j][h].x, acc[4 * h]);
+        acc[4 * h + 1] = fmaf(w[j], v[j][h].y, acc[4 * h + 1]);
+        acc[4 * h + 2] = fmaf(w[j], v[j][h].z, acc[4 * h + 2]);
+        acc[4 * h + 3] = fmaf(w[j], v[j][h].w, acc[4 * h + 3]);
+      }
+  }
+  if (!live) return;
+  const float rl = total != 0.f ? __frcp_rn(total) : 0.f;
+  *reinterpret_cast<uint4*>(p.out + r * kDimLatent + col) =
+      make_uint4(pack_bf16x2(acc[0] * rl, acc[1] * rl), pack_bf16x2(acc[2] * rl, acc[3] * rl),
+                 pack_bf16x2(acc[4] * rl, acc[5] * rl), pack_bf16x2(acc[6] * rl, acc[7] * rl));
+  if (col == 0) {
     p.out_max[r] = total != 0.f ? top : -INFINITY;
     p.out_sum[r] = total;
   }
@@ -722,17 +801,29 @@ cudaError_t launch_fwd_prefix(const PrefixParams& p, const void* kv, const void*
   Maps maps;
   if (!encode(&maps.half, kv, p.keys, 8, 4) || !encode(&maps.rope, k_rope, p.keys, 1, 1))
     return cudaErrorInvalidValue;
+  PrefixParams scaled = p;
+  scaled.scale_div = (float)(p.scale_div * (1.0 - kCutBias));
+  scaled.scale_log2 = (float)(p.scale_log2 * (1.0 + kCutBias));
   const long long items = (p.rows + kPxRows - 1) / kPxRows * p.split;
   if (items <= 0 || 2 * items > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
   cudaLaunchConfig_t cfg;
   cudaLaunchAttribute attr;
   if (!launch_config(&cfg, &attr, (unsigned)(2 * items), stream)) return cudaErrorInvalidConfiguration;
-  return cudaLaunchKernelEx(&cfg, fwd_prefix_kernel, p, maps);
+  return cudaLaunchKernelEx(&cfg, fwd_prefix_kernel, scaled, maps);
 }
 
 cudaError_t launch_prefix_join(const JoinParams& p, cudaStream_t stream) {
-  prefix_join_kernel<<<(unsigned)((p.rows + 7) / 8), 256, 0, stream>>>(p);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;  // its start overlaps the end of the kernel before it
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  if (p.split + p.own_split > kJoinMaxParts) return cudaErrorInvalidValue;
+  cfg.gridDim = dim3((unsigned)((p.rows + 31) / 32), kDimLatent / (8 * kJoinWarps), 1);
+  cfg.blockDim = dim3(32 * kJoinWarps, 1, 1);
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, prefix_join_kernel, p);
 }
 
 }  // namespace dsa

@@ -517,6 +517,7 @@ __global__ void __launch_bounds__(kStThreads, 2) fwd_stream_kernel(const FwdPara
     }
   }
   if (failed && ctid == 0) report_error(p.status, kErrTimeout);
+  if (p.beside_previous && blockIdx.x == gridDim.x - 1) grid_dependency_wait();
   if constexpr (kCM) stream_cluster_merge(p, !(*abort_flag) && !*reinterpret_cast<volatile int*>(&sm.stop));
 }
 
@@ -602,7 +603,21 @@ cudaError_t launch_fwd_stream(const FwdParams& p, cudaStream_t stream, bool merg
   }
   const int max_ctas = stream_max_ctas();
   if (max_ctas <= 0) return cudaErrorInvalidConfiguration;
-  const int ctas = (int)(items < max_ctas ? items : max_ctas);
+  // beside another kernel: a CTA per item, which start as SMs become free
+  const int ctas = (int)(p.beside_previous || items < max_ctas ? items : max_ctas);
+  if (p.beside_previous) {
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3((unsigned)ctas, 1, 1);
+    cfg.blockDim = dim3(kStThreads, 1, 1);
+    cfg.dynamicSmemBytes = sizeof(StSmem);
+    cfg.stream = stream;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, fwd_stream_kernel<false>, p);
+  }
   fwd_stream_kernel<false><<<ctas, kStThreads, sizeof(StSmem), stream>>>(p);
   return cudaGetLastError();
 }

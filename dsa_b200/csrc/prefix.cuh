@@ -12,7 +12,7 @@ struct PrefixParams {
   __nv_bfloat16* out;           // without partials: [rows, 512], [rows], [rows]
   float* out_max;
   float* out_sum;
-  float* part_num;              // [row tiles, split, 128, 512], or null: write the output
+  float* part_num;              // [row tiles, split, 512 / 8, 128, 8] (groups of 8 columns), or null: write the output
   float* part_max;              // [row tiles, split, 128]
   float* part_sum;
   int32_t* status;
