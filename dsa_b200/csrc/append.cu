@@ -9,8 +9,9 @@
 // distinct (a page plan's are).
 //
 // Bound: HBM, 1152 bytes read and 1152 (656) written per token; one warp per
-// token, a lane's 16 latent values are two 16-byte loads, a 128-dim block is
-// eight lanes (three shuffles for its maximum) and lane i turns pair i.
+// token at a time, a lane's 16 latent values are two 16-byte loads, a 128-dim
+// block is eight lanes (three shuffles for its maximum) and lane i turns pair i,
+// whose turn fraction it keeps.
 #include <cuda_fp8.h>
 
 #include "serving.cuh"
@@ -36,63 +37,124 @@ __device__ __forceinline__ void load16(const __nv_bfloat16* src, uint4& a, uint4
   }
 }
 
+__device__ __forceinline__ uint32_t pack_e4m3(const float* x) {
+  return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(x[0], x[1]), __NV_SATFINITE, __NV_E4M3) |
+         ((uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(x[2], x[3]), __NV_SATFINITE, __NV_E4M3) << 16);
+}
+
+// One token's row as a lane holds it.
+struct Row {
+  uint4 v0, v1;          // 16 latent values
+  __nv_bfloat16 r0, r1;  // a pair of rope values
+  int32_t pos;
+};
+
 // kWide: kv rows start on 16-byte boundaries.
-template <bool kFp8, bool kWide>
-__global__ void __launch_bounds__(kApThreads) append_kernel(const AppendParams p) {
-  const int lane = threadIdx.x & 31;
-  const long long stride = (long long)gridDim.x * (kApThreads / 32);
-  // this lane's pair of rope dims and its frequency
-  const int e0 = p.half ? lane : 2 * lane, e1 = p.half ? lane + 32 : 2 * lane + 1;
-  const double freq = p.inv_freq != nullptr ? __ldg(p.inv_freq + lane) : 0.0;
-  for (long long t = (long long)blockIdx.x * (kApThreads / 32) + (threadIdx.x >> 5); t < p.tokens; t += stride) {
-    const long long slot = __ldg(p.slots + t);
-    if (slot < 0 || slot >= p.rows) continue;
-    const int b = (int)(t / p.queries), s = (int)(t - (long long)b * p.queries);
-    const __nv_bfloat16* const kv = p.kv + b * p.kvs[0] + s * p.kvs[1];
-    const __nv_bfloat16* const kr = p.k_rope + b * p.krs[0] + s * p.krs[1];
-    uint4 v0, v1;
-    load16<kWide>(kv + lane * 16, v0, v1);
-    __nv_bfloat16 r0 = kr[e0], r1 = kr[e1];
-    if (p.inv_freq != nullptr) {
-      float c, sn;
-      rotary_cos_sin(__ldg(p.positions + t), freq, p.factor, 1.f, &c, &sn);
-      const float2 turned = rotate_pair(__bfloat162float(r0), __bfloat162float(r1), c, sn);
-      r0 = __float2bfloat16_rn(turned.x);
-      r1 = __float2bfloat16_rn(turned.y);
-    }
-    __nv_bfloat16* rope;
-    if (kFp8) {
-      uint8_t* const row = p.cache + slot * kApRowBytes;
-      const uint32_t w[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
-      // |bits| order as the magnitudes do, a NaN above every number
-      uint32_t top = 0;
+template <bool kWide>
+__device__ __forceinline__ void load_row(const AppendParams& p, uint32_t t, int lane, int e0, int e1, Row& r) {
+  const uint32_t b = t / (uint32_t)p.queries, s = t - b * (uint32_t)p.queries;
+  const __nv_bfloat16* const kr = p.k_rope + b * p.krs[0] + s * p.krs[1];
+  load16<kWide>(p.kv + b * p.kvs[0] + s * p.kvs[1] + lane * 16, r.v0, r.v1);
+  r.r0 = kr[e0];
+  r.r1 = kr[e1];
+  r.pos = p.positions != nullptr ? __ldg(p.positions + t) : 0;
+}
+
+template <bool kFp8>
+__device__ __forceinline__ void write_row(const AppendParams& p, long long slot, int lane, int e0, int e1,
+                                          unsigned long long fraction, Row& r) {
+  if (p.inv_freq != nullptr) {
+    float c, sn;
+    rotary_cos_sin(r.pos, fraction, p.factor, 1.f, &c, &sn);
+    const float2 turned = rotate_pair(__bfloat162float(r.r0), __bfloat162float(r.r1), c, sn);
+    r.r0 = __float2bfloat16_rn(turned.x);
+    r.r1 = __float2bfloat16_rn(turned.y);
+  }
+  __nv_bfloat16* rope;
+  if (kFp8) {
+    uint8_t* const row = p.cache + slot * kApRowBytes;
+    const uint32_t w[8] = {r.v0.x, r.v0.y, r.v0.z, r.v0.w, r.v1.x, r.v1.y, r.v1.z, r.v1.w};
+    // |bits| order as the magnitudes do, a NaN above every number
+    uint32_t both = 0;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) top = max(top, max(w[k] & 0x7fffu, (w[k] >> 16) & 0x7fffu));
+    for (int k = 0; k < 8; ++k) both = __vmaxu2(both, w[k] & 0x7fff7fffu);
+    uint32_t top = max(both & 0xffffu, both >> 16);
 #pragma unroll
-      for (int d = 1; d < 8; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
-      const float amax = __uint_as_float(top << 16);
-      const float scale = amax > 0.f ? __fdiv_rn(amax, 448.f) : 1.f;
-      uint32_t q[4];
+    for (int d = 1; d < 8; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+    const float amax = __uint_as_float(top << 16);
+    const float scale = amax > 0.f ? __fdiv_rn(amax, 448.f) : 1.f;
+    // kv / scale, correctly rounded: with the correctly rounded reciprocal one
+    // Newton step on the quotient's exact remainder gives it (Markstein, 1990)
+    // while nothing leaves the normal range; 16 divisions would cost a lane
+    // more than all the rest.
+    uint32_t q[4];
+    if (scale >= 0x1p-60f && scale <= 0x1p60f) {
+      const float inv = __frcp_rn(scale);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const float2 lo = make_float2(__fdiv_rn(__uint_as_float(w[2 * k] << 16), scale),
-                                      __fdiv_rn(__uint_as_float(w[2 * k] & 0xffff0000u), scale));
-        const float2 hi = make_float2(__fdiv_rn(__uint_as_float(w[2 * k + 1] << 16), scale),
-                                      __fdiv_rn(__uint_as_float(w[2 * k + 1] & 0xffff0000u), scale));
-        q[k] = (uint32_t)__nv_cvt_float2_to_fp8x2(lo, __NV_SATFINITE, __NV_E4M3) |
-               ((uint32_t)__nv_cvt_float2_to_fp8x2(hi, __NV_SATFINITE, __NV_E4M3) << 16);
+        float x[4] = {__uint_as_float(w[2 * k] << 16), __uint_as_float(w[2 * k] & 0xffff0000u),
+                      __uint_as_float(w[2 * k + 1] << 16), __uint_as_float(w[2 * k + 1] & 0xffff0000u)};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float y = __fmul_rn(x[i], inv);
+          x[i] = __fmaf_rn(__fmaf_rn(-y, scale, x[i]), inv, y);
+        }
+        q[k] = pack_e4m3(x);
       }
-      reinterpret_cast<uint4*>(row)[lane] = make_uint4(q[0], q[1], q[2], q[3]);
-      if ((lane & 7) == 0) reinterpret_cast<float*>(row + kDimLatent)[lane >> 3] = scale;
-      rope = reinterpret_cast<__nv_bfloat16*>(row + kDimLatent + 16);
     } else {
-      uint4* const dst = reinterpret_cast<uint4*>(p.kv_cache + slot * kDimLatent) + 2 * lane;
-      dst[0] = v0;
-      dst[1] = v1;
-      rope = p.rope_cache + slot * kDimRope;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float x[4] = {__fdiv_rn(__uint_as_float(w[2 * k] << 16), scale),
+                            __fdiv_rn(__uint_as_float(w[2 * k] & 0xffff0000u), scale),
+                            __fdiv_rn(__uint_as_float(w[2 * k + 1] << 16), scale),
+                            __fdiv_rn(__uint_as_float(w[2 * k + 1] & 0xffff0000u), scale)};
+        q[k] = pack_e4m3(x);
+      }
     }
-    rope[e0] = r0;
-    rope[e1] = r1;
+    reinterpret_cast<uint4*>(row)[lane] = make_uint4(q[0], q[1], q[2], q[3]);
+    if ((lane & 7) == 0) reinterpret_cast<float*>(row + kDimLatent)[lane >> 3] = scale;
+    rope = reinterpret_cast<__nv_bfloat16*>(row + kDimLatent + 16);
+  } else {
+    uint4* const dst = reinterpret_cast<uint4*>(p.kv_cache + slot * kDimLatent) + 2 * lane;
+    dst[0] = r.v0;
+    dst[1] = r.v1;
+    rope = p.rope_cache + slot * kDimRope;
+  }
+  if (e1 == e0 + 1) {
+    __nv_bfloat162 pair;
+    pair.x = r.r0;
+    pair.y = r.r1;
+    *reinterpret_cast<__nv_bfloat162*>(rope + e0) = pair;
+  } else {
+    rope[e0] = r.r0;
+    rope[e1] = r.r1;
+  }
+}
+
+// A warp walks over tokens; the next token's row and the slot of the one after
+// it are under way while a row is written.
+template <bool kFp8, bool kWide>
+__global__ void __launch_bounds__(kApThreads, 5) append_kernel(const AppendParams p) {
+  const int lane = threadIdx.x & 31;
+  const uint32_t stride = gridDim.x * (kApThreads / 32);
+  const uint32_t tokens = (uint32_t)p.tokens;  // < 2^31
+  const int e0 = p.half ? lane : 2 * lane, e1 = p.half ? lane + 32 : 2 * lane + 1;
+  const unsigned long long fraction = p.inv_freq != nullptr ? turn_fraction(__ldg(p.inv_freq + lane)) : 0;
+  auto slot_of = [&](uint32_t t) -> long long {
+    const int32_t slot = t < tokens ? __ldg(p.slots + t) : -1;
+    return slot < p.rows ? slot : -1;
+  };
+  uint32_t t = blockIdx.x * (kApThreads / 32) + (threadIdx.x >> 5);
+  long long slot = slot_of(t), slot_nx = slot_of(t + stride);
+  Row cur, nx;
+  if (slot >= 0) load_row<kWide>(p, t, lane, e0, e1, cur);
+  for (; t < tokens; t += stride) {
+    const long long slot_nx2 = slot_of(t + 2 * stride);
+    if (slot_nx >= 0) load_row<kWide>(p, t + stride, lane, e0, e1, nx);
+    if (slot >= 0) write_row<kFp8>(p, slot, lane, e0, e1, fraction, cur);
+    slot = slot_nx;
+    slot_nx = slot_nx2;
+    cur = nx;
   }
 }
 
@@ -100,7 +162,7 @@ __global__ void __launch_bounds__(kApThreads) append_kernel(const AppendParams p
 
 cudaError_t launch_append_kv(const AppendParams& p, cudaStream_t stream) {
   long long blocks = (p.tokens + kApThreads / 32 - 1) / (kApThreads / 32);
-  if (blocks > 148 * 8 * 4) blocks = 148 * 8 * 4;
+  if (blocks > 148 * 5) blocks = 148 * 5;
   bool wide = (reinterpret_cast<uintptr_t>(p.kv) & 15u) == 0 && p.kvs[0] % 8 == 0 && p.kvs[1] % 8 == 0;
   const unsigned g = (unsigned)blocks;
   if (p.cache != nullptr) {

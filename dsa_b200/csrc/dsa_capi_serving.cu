@@ -110,7 +110,7 @@ int dsa_rotary(const dsa_rotary_args_t* a, void* stream) {
   if (a == nullptr || !a->x || !a->y || !a->positions || !a->inv_freq) return DSA_STATUS_BAD_ARGUMENT;
   if (!product_ok(a->batch, a->queries) || a->heads <= 0 || a->heads > kMaxInt || a->dim <= 0 || a->dim > 65536)
     return DSA_STATUS_BAD_ARGUMENT;
-  if (a->rotary_dim <= 0 || a->rotary_dim % 2 != 0 || a->start < 0 || a->start > a->dim - a->rotary_dim)
+  if (a->rotary_dim <= 0 || a->rotary_dim > 8192 || a->rotary_dim % 2 != 0 || a->start < 0 || a->start > a->dim - a->rotary_dim)
     return DSA_STATUS_BAD_ARGUMENT;
   if (a->dtype < DSA_BF16 || a->dtype > DSA_FP32 || (a->layout != DSA_ROPE_INTERLEAVED && a->layout != DSA_ROPE_HALF))
     return DSA_STATUS_BAD_ARGUMENT;

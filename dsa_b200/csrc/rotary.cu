@@ -6,12 +6,13 @@
 // (half). The other elements are copied. The gradient of y with respect to x
 // is the same map with -t, so the backward pass is this kernel again.
 //
-// Bound: HBM, 2 * dim elements per head row. The cosines cost ~40 FP32 and 5
-// FP64 instructions a pair, more than the memory time of one row, and depend
-// on the token alone: a thread owns fixed pairs of one token and walks over
-// heads h, h + groups, ..., so they are computed once per thread and stay in
-// registers. A unit is two 16-byte vectors half the turned part apart: with
-// that split both layouts load whole contiguous lines per warp.
+// Bound: HBM, 2 * dim elements per head row. The cosines cost ~50 instructions
+// a pair, more than the memory time of one row, and depend
+// on the token alone: a block computes those of its tokens once into shared
+// memory, while its first loads are under way, and a thread walks over heads
+// h, h + groups, ... with its pairs' cosines in registers. A unit is two
+// 16-byte vectors half the turned part apart: with that split both layouts
+// load whole contiguous lines per warp.
 #include <cuda_fp16.h>
 
 #include "serving.cuh"
@@ -20,111 +21,172 @@ namespace dsa {
 namespace {
 
 constexpr int kRoThreads = 256;
+constexpr int kRoTable = 2048;  // cosine pairs of a block
 
+// The two 16-bit numbers of a word, and back (one rounding each).
 template <typename T>
-__device__ __forceinline__ float to_f(T v);
+__device__ __forceinline__ float2 unpack(uint32_t w);
 template <>
-__device__ __forceinline__ float to_f(float v) { return v; }
+__device__ __forceinline__ float2 unpack<__nv_bfloat16>(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
 template <>
-__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
-template <>
-__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float2 unpack<__half>(uint32_t w) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
 template <typename T>
-__device__ __forceinline__ T from_f(float v);
+__device__ __forceinline__ uint32_t pack(float lo, float hi);
 template <>
-__device__ __forceinline__ float from_f(float v) { return v; }
+__device__ __forceinline__ uint32_t pack<__nv_bfloat16>(float lo, float hi) { return pack_bf16x2(lo, hi); }
 template <>
-__device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __float2bfloat16_rn(v); }
+__device__ __forceinline__ uint32_t pack<__half>(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
 
-// V elements of T loaded and stored as one access.
+// Two vectors of V elements of one head: 16 bytes each (V > 1), or one
+// element each. turn() maps the pairs they hold: with the half layout a pair
+// has an element in either; interleaved, each vector holds V / 2 pairs (with
+// one element a vector the two are the pair).
 template <typename T, int V>
-struct alignas(sizeof(T) * V) Vec {
-  T e[V];
+struct Two {
+  uint32_t a[4], d[4];
+  __device__ __forceinline__ void load(const T* x, int o0, int o1, bool two) {
+    const uint4 v = *reinterpret_cast<const uint4*>(x + o0);
+    a[0] = v.x, a[1] = v.y, a[2] = v.z, a[3] = v.w;
+    if (two) {
+      const uint4 w = *reinterpret_cast<const uint4*>(x + o1);
+      d[0] = w.x, d[1] = w.y, d[2] = w.z, d[3] = w.w;
+    }
+  }
+  __device__ __forceinline__ void store(T* y, int o0, int o1, bool two) const {
+    *reinterpret_cast<uint4*>(y + o0) = make_uint4(a[0], a[1], a[2], a[3]);
+    if (two) *reinterpret_cast<uint4*>(y + o1) = make_uint4(d[0], d[1], d[2], d[3]);
+  }
+  template <bool kHalf>
+  __device__ __forceinline__ void turn(const float2* cs) {
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 x0 = unpack<T>(a[k]), x1 = unpack<T>(d[k]);
+        if constexpr (kHalf) {
+          const float2 p0 = rotate_pair(x0.x, x1.x, cs[2 * k].x, cs[2 * k].y);
+          const float2 p1 = rotate_pair(x0.y, x1.y, cs[2 * k + 1].x, cs[2 * k + 1].y);
+          a[k] = pack<T>(p0.x, p1.x);
+          d[k] = pack<T>(p0.y, p1.y);
+        } else {
+          const float2 p0 = rotate_pair(x0.x, x0.y, cs[k].x, cs[k].y);
+          const float2 p1 = rotate_pair(x1.x, x1.y, cs[4 + k].x, cs[4 + k].y);
+          a[k] = pack<T>(p0.x, p0.y);
+          d[k] = pack<T>(p1.x, p1.y);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; k += kHalf ? 1 : 2) {
+        if constexpr (kHalf) {
+          const float2 p0 = rotate_pair(__uint_as_float(a[k]), __uint_as_float(d[k]), cs[k].x, cs[k].y);
+          a[k] = __float_as_uint(p0.x);
+          d[k] = __float_as_uint(p0.y);
+        } else {
+          const float2 p0 = rotate_pair(__uint_as_float(a[k]), __uint_as_float(a[k + 1]), cs[k / 2].x, cs[k / 2].y);
+          const float2 p1 = rotate_pair(__uint_as_float(d[k]), __uint_as_float(d[k + 1]), cs[2 + k / 2].x, cs[2 + k / 2].y);
+          a[k] = __float_as_uint(p0.x), a[k + 1] = __float_as_uint(p0.y);
+          d[k] = __float_as_uint(p1.x), d[k + 1] = __float_as_uint(p1.y);
+        }
+      }
+    }
+  }
+};
+template <typename T>
+struct Two<T, 1> {
+  T a, d;
+  __device__ __forceinline__ void load(const T* x, int o0, int o1, bool two) {
+    a = x[o0];
+    if (two) d = x[o1];
+  }
+  __device__ __forceinline__ void store(T* y, int o0, int o1, bool two) const {
+    y[o0] = a;
+    if (two) y[o1] = d;
+  }
+  template <bool kHalf>
+  __device__ __forceinline__ void turn(const float2* cs) {
+    const float2 p = rotate_pair((float)a, (float)d, cs[0].x, cs[0].y);
+    a = (T)p.x;
+    d = (T)p.y;
+  }
 };
 
 // V: elements of a vector (16 bytes' worth, or 1 for sizes, strides or
 // addresses that 16-byte accesses do not fit).
-template <typename T, int V>
+template <typename T, int V, bool kHalf>
 __global__ void __launch_bounds__(kRoThreads) rotary_kernel(const RotaryParams p, int groups, int units_rot,
                                                             int units, int tokens_per_block) {
-  using VT = Vec<T, V>;
+  extern __shared__ float2 table[];  // [tokens of the block][rotary_dim / 2], then turn fractions and positions
   const int per_token = groups * units;
-  long long token;
-  int w;
-  if (tokens_per_block > 1) {
-    const int k = threadIdx.x / per_token;
-    if (k >= tokens_per_block) return;
-    token = (long long)blockIdx.x * tokens_per_block + k;
-    w = threadIdx.x - k * per_token;
-  } else {
-    token = blockIdx.x;
-    w = blockIdx.y * kRoThreads + threadIdx.x;
-  }
-  if (token >= p.tokens || w >= per_token) return;
+  const int k = tokens_per_block > 1 ? (int)threadIdx.x / per_token : 0;
+  const long long token = (long long)blockIdx.x * tokens_per_block + k;
+  const int w = tokens_per_block > 1 ? (int)threadIdx.x - k * per_token : (int)(blockIdx.y * kRoThreads + threadIdx.x);
+  const bool live = k < tokens_per_block && token < p.tokens && w < per_token;
   const int g = w / units, u = w - g * units;
-  const int b = (int)(token / p.queries), s = (int)(token - (long long)b * p.queries);
-  const T* const x = static_cast<const T*>(p.x) + b * p.xs[0] + s * p.xs[1];
-  T* const y = static_cast<T*>(p.y) + b * p.ys[0] + s * p.ys[1];
+  const uint32_t b = live ? (uint32_t)token / (uint32_t)p.queries : 0u;  // tokens < 2^31
+  const uint32_t s = live ? (uint32_t)token - b * (uint32_t)p.queries : 0u;
+  const T* x = static_cast<const T*>(p.x) + b * p.xs[0] + s * p.xs[1] + g * p.xs[2];
+  T* y = static_cast<T*>(p.y) + b * p.ys[0] + s * p.ys[1] + g * p.ys[2];
 
-  if (u >= units_rot) {  // copied elements: vectors c and c + units_copy
-    const int vecs = (p.dim - p.rotary_dim) / V, first = p.start / V, units_copy = units - units_rot;
-    int c0 = u - units_rot, c1 = c0 + units_copy;
-    const bool two = c1 < vecs;
-    const int skip = p.rotary_dim / V;
-    c0 += c0 >= first ? skip : 0;
-    c1 += c1 >= first ? skip : 0;
-#pragma unroll 4
-    for (int h = g; h < p.heads; h += groups) {
-      const T* const xh = x + h * p.xs[2];
-      T* const yh = y + h * p.ys[2];
-      const VT v0 = *reinterpret_cast<const VT*>(xh + c0 * V);
-      if (two) *reinterpret_cast<VT*>(yh + c1 * V) = *reinterpret_cast<const VT*>(xh + c1 * V);
-      *reinterpret_cast<VT*>(yh + c0 * V) = v0;
-    }
-    return;
+  // this thread's two vectors: of a rotary unit, or copied ones
+  const bool turns = u < units_rot;
+  int o0, o1;
+  bool two = true;
+  if (turns) {
+    o0 = p.start + (V == 1 && !kHalf ? 2 * u : u * V);
+    o1 = V == 1 && !kHalf ? o0 + 1 : o0 + p.rotary_dim / 2;
+  } else {
+    const int vecs = (p.dim - p.rotary_dim) / V, first = p.start / V, skip = p.rotary_dim / V;
+    const int c0 = u - units_rot, c1 = c0 + units - units_rot;
+    two = c1 < vecs;
+    o0 = (c0 + (c0 >= first ? skip : 0)) * V;
+    o1 = (c1 + (c1 >= first ? skip : 0)) * V;
   }
+  Two<T, V> cur;
+  if (live) cur.load(x, o0, o1, two);
 
-  // this thread's V pairs: with V > 1 and interleaved pairs, V / 2 in each of
-  // its two vectors
-  const long long pos = p.pos64 ? static_cast<const long long*>(p.positions)[b * p.ps[0] + s * p.ps[1]]
-                                : (long long)static_cast<const int32_t*>(p.positions)[b * p.ps[0] + s * p.ps[1]];
-  const int o0 = p.start + (V == 1 && !p.half ? 2 * u : u * V);
-  const int o1 = V == 1 && !p.half ? o0 + 1 : o0 + p.rotary_dim / 2;
-  float c[V], sn[V];
-#pragma unroll
-  for (int k = 0; k < V; ++k) {
-    int i = u * V + k;
-    if (V > 1 && !p.half) i = k < V / 2 ? u * (V / 2) + k : p.rotary_dim / 4 + u * (V / 2) + k - V / 2;
-    rotary_cos_sin(pos, __ldg(p.inv_freq + i), p.factor, p.sin_sign, &c[k], &sn[k]);
+  const int pairs = p.rotary_dim / 2;
+  unsigned long long* const fraction = reinterpret_cast<unsigned long long*>(table + tokens_per_block * pairs);
+  long long* const position = reinterpret_cast<long long*>(fraction + pairs);
+  for (int j = threadIdx.x; j < pairs; j += kRoThreads) fraction[j] = turn_fraction(__ldg(p.inv_freq + j));
+  if (threadIdx.x < tokens_per_block) {  // at most kRoThreads
+    const uint32_t t = (uint32_t)min((long long)blockIdx.x * tokens_per_block + threadIdx.x, p.tokens - 1);
+    const uint32_t tb = t / (uint32_t)p.queries, ts = t - tb * (uint32_t)p.queries;
+    const long long at = tb * p.ps[0] + ts * p.ps[1];
+    position[threadIdx.x] = p.pos64 ? static_cast<const long long*>(p.positions)[at]
+                                    : (long long)static_cast<const int32_t*>(p.positions)[at];
   }
-  const bool across = V == 1 || p.half;  // a pair's elements are in different vectors
-#pragma unroll 4
-  for (int h = g; h < p.heads; h += groups) {
-    const VT a = *reinterpret_cast<const VT*>(x + h * p.xs[2] + o0);
-    const VT d = *reinterpret_cast<const VT*>(x + h * p.xs[2] + o1);
-    VT ra, rd;
-    if (across) {
+  __syncthreads();
+  for (int i = threadIdx.x; i < tokens_per_block * pairs; i += kRoThreads) {
+    const int tk = i / pairs, j = i - tk * pairs;
+    rotary_cos_sin(position[tk], fraction[j], p.factor, p.sin_sign, &table[i].x, &table[i].y);
+  }
+  __syncthreads();
+  if (!live) return;
+
+  const long long xstep = groups * p.xs[2], ystep = groups * p.ys[2];
+  float2 cs[V];
+  if (turns) {
 #pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const float2 t = rotate_pair(to_f(a.e[k]), to_f(d.e[k]), c[k], sn[k]);
-        ra.e[k] = from_f<T>(t.x);
-        rd.e[k] = from_f<T>(t.y);
-      }
-    } else {
-#pragma unroll
-      for (int k = 0; k < V / 2; ++k) {
-        const float2 t = rotate_pair(to_f(a.e[2 * k]), to_f(a.e[2 * k + 1]), c[k], sn[k]);
-        const float2 v = rotate_pair(to_f(d.e[2 * k]), to_f(d.e[2 * k + 1]), c[k + V / 2], sn[k + V / 2]);
-        ra.e[2 * k] = from_f<T>(t.x);
-        ra.e[2 * k + 1] = from_f<T>(t.y);
-        rd.e[2 * k] = from_f<T>(v.x);
-        rd.e[2 * k + 1] = from_f<T>(v.y);
-      }
-    }
-    *reinterpret_cast<VT*>(y + h * p.ys[2] + o0) = ra;
-    *reinterpret_cast<VT*>(y + h * p.ys[2] + o1) = rd;
+    for (int q = 0; q < V; ++q)
+      cs[q] = table[k * pairs + (V == 1 || kHalf ? u * V + q
+                                                 : q < V / 2 ? u * (V / 2) + q : p.rotary_dim / 4 + u * (V / 2) + q - V / 2)];
+  }
+  for (int h = g;;) {  // the next head's loads are under way while this one is turned
+    Two<T, V> next;
+    const bool more = (h += groups) < p.heads;
+    if (more) next.load(x += xstep, o0, o1, two);
+    if (turns) cur.template turn<kHalf>(cs);
+    cur.store(y, o0, o1, two);
+    if (!more) return;
+    y += ystep;
+    cur = next;
   }
 }
 
@@ -133,9 +195,10 @@ cudaError_t launch_v(const RotaryParams& p, cudaStream_t stream) {
   const int units_rot = p.rotary_dim / (2 * V);
   const int copies = p.in_place ? 0 : (p.dim - p.rotary_dim) / V;
   const int units = units_rot + (copies + 1) / 2;
-  // heads per thread: one while that leaves a part of the GPU idle (148 SMs
-  // x 2048 threads), then as many as keep the GPU full, so that a thread's
-  // cosines serve more rows
+  // heads per thread: one while that leaves a part of the GPU idle, then as
+  // many as keep it full (148 SMs x 2048 threads), so that a block's cosines
+  // serve more rows. 4096 tokens x 64 heads x 128 (64 turned): 23.4 us, with
+  // half as many threads 24.4, with four times as many 29.3.
   const long long want = 148LL * 2048;
   long long groups = (want + p.tokens * units - 1) / (p.tokens * units);
   if (groups > p.heads) groups = p.heads;
@@ -144,10 +207,13 @@ cudaError_t launch_v(const RotaryParams& p, cudaStream_t stream) {
   const long long per_token = groups * units;
   if (per_token > 0x7fffffffLL / 2) return cudaErrorInvalidConfiguration;
   int tpb = per_token < kRoThreads ? (int)(kRoThreads / per_token) : 1;
+  if (tpb > kRoTable / (p.rotary_dim / 2)) tpb = kRoTable / (p.rotary_dim / 2) > 0 ? kRoTable / (p.rotary_dim / 2) : 1;
   dim3 grid((unsigned)((p.tokens + tpb - 1) / tpb), 1, 1);
   if (tpb == 1) grid.y = (unsigned)((per_token + kRoThreads - 1) / kRoThreads);
-  if (grid.y > 65535) return cudaErrorInvalidConfiguration;
-  rotary_kernel<T, V><<<grid, kRoThreads, 0, stream>>>(p, (int)groups, units_rot, units, tpb);
+  if (tpb < 1 || grid.y > 65535) return cudaErrorInvalidConfiguration;
+  const size_t smem = (size_t)(tpb + 1) * (p.rotary_dim / 2) * sizeof(float2) + (size_t)tpb * sizeof(long long);
+  if (p.half) rotary_kernel<T, V, true><<<grid, kRoThreads, smem, stream>>>(p, (int)groups, units_rot, units, tpb);
+  else rotary_kernel<T, V, false><<<grid, kRoThreads, smem, stream>>>(p, (int)groups, units_rot, units, tpb);
   return cudaGetLastError();
 }
 

@@ -60,16 +60,31 @@ struct AppendParams {
 cudaError_t launch_append_kv(const AppendParams& p, cudaStream_t stream);
 
 #ifdef __CUDACC__
-// factor * (cos, sin) of the angle pos * freq. The angle is counted in turns
-// in FP64 and reduced there: an FP32 angle of position 10^6 would be off by
-// up to 2^-5 radians, the reduced one is within 2^-24 of a half turn for
-// every 32-bit position.
-__device__ __forceinline__ void rotary_cos_sin(long long pos, double freq, float factor, float sin_sign, float* c,
-                                               float* s) {
-  double t = (double)pos * freq * 0.15915494309189533577;  // 1 / (2 pi)
-  t -= rint(t);
+// freq / (2 pi), radians to turns a position, modulo one turn as a 64-bit
+// fraction: positions are integers, so whole turns of the frequency do not
+// matter, and position * fraction modulo 2^64 is the angle in turns, reduced
+// exactly. 1 / (2 pi) and the product are taken in two FP64 pieces; the
+// fraction is off by 2^-64 of a turn, the angle of position 2^31 by 2^-33.
+__device__ __forceinline__ unsigned long long turn_fraction(double freq) {
+  constexpr double kInvTwoPi = 0.15915494309189535, kInvTwoPiLo = -9.839338337591243e-18;
+  const double hi = freq * kInvTwoPi;
+  double lo = fma(freq, kInvTwoPi, -hi) + freq * kInvTwoPiLo;
+  double t = hi - floor(hi);                      // exact
+  // 2^32 t = whole + rest; the small piece joins the rest
+  const double w = floor(t * 4294967296.0);
+  lo = (t * 4294967296.0 - w) + lo * 4294967296.0;
+  return ((unsigned long long)w << 32) + (unsigned long long)(long long)rint(lo * 4294967296.0);
+}
+
+// factor * (cos, sin) of position pos; the angle rounds to 2^-24 of a half turn
+// (an FP32 angle of position 10^6 would be off by up to 2^-5 radians). Three
+// integer products instead of five FP64 instructions and two conversions, which
+// bound the rotation of single heads.
+__device__ __forceinline__ void rotary_cos_sin(long long pos, unsigned long long fraction, float factor, float sin_sign,
+                                               float* c, float* s) {
+  const int half_turns = (int)(((unsigned long long)pos * fraction) >> 32);
   float sn, cs;
-  sincospif((float)(t + t), &sn, &cs);
+  sincospif((float)half_turns * 0x1p-31f, &sn, &cs);
   *c = cs * factor;
   *s = sn * (factor * sin_sign);
 }

@@ -119,7 +119,12 @@ class _Rotary(torch.autograd.Function):
         number, start, factor, inverse = ctx.how
         if grad.stride(-1) != 1:
             grad = grad.contiguous()
-        return _Rotary.apply(grad, positions, inv_freq, number, start, factor, not inverse), None, None, None, None, None, None
+        if torch.is_grad_enabled():  # a graph of the gradient is wanted
+            gx = _Rotary.apply(grad, positions, inv_freq, number, start, factor, not inverse)
+        else:
+            gx = _launch(grad, positions, inv_freq, torch.empty(grad.shape, dtype=grad.dtype, device=grad.device), number,
+                         start, factor, not inverse)
+        return gx, None, None, None, None, None, None
 
 
 def rotary(x, positions, inv_freq, *, layout="interleaved", start=0, attention_factor=1.0, inverse=False, out=None):
@@ -153,6 +158,8 @@ def rotary(x, positions, inv_freq, *, layout="interleaved", start=0, attention_f
     turned, dim = 2 * inv_freq.shape[0], shape[-1]
     if type(start) is not int or start < 0 or turned == 0 or start + turned > dim:
         raise ValueError("need 0 <= start and start + 2 * len(inv_freq) <= D")
+    if turned > 8192 or dim > 65536:
+        raise ValueError("at most 8192 turned elements of a row of at most 65536")
     if x.stride(-1) != 1:
         raise ValueError("the last dimension of x must be contiguous")
     inverse = bool(inverse)
