@@ -46,7 +46,8 @@ int prefix_split(int64_t row_tiles, int64_t keys, int clusters) {
   const int64_t tiles = (keys + 63) / 64;
   double best = 0;
   int split = 1;
-  for (int s = 1; s <= 128 && s <= tiles; ++s) {
+  // more than four waves of items never pay
+  for (int s = 1; s <= 128 && s <= tiles && (s == 1 || row_tiles * s <= 4 * (int64_t)clusters); ++s) {
     const int64_t waves = (row_tiles * s + clusters - 1) / clusters;
     const double us = 0.6 * (double)waves * (double)((tiles + s - 1) / s + 6) +
                       (s > 1 ? (double)row_tiles * s * 128 * 4096 / 5e6 : 0.0);
@@ -110,7 +111,7 @@ int dsa_rotary(const dsa_rotary_args_t* a, void* stream) {
   if (a == nullptr || !a->x || !a->y || !a->positions || !a->inv_freq) return DSA_STATUS_BAD_ARGUMENT;
   if (!product_ok(a->batch, a->queries) || a->heads <= 0 || a->heads > kMaxInt || a->dim <= 0 || a->dim > 65536)
     return DSA_STATUS_BAD_ARGUMENT;
-  if (a->rotary_dim <= 0 || a->rotary_dim > 8192 || a->rotary_dim % 2 != 0 || a->start < 0 || a->start > a->dim - a->rotary_dim)
+  if (a->rotary_dim <= 0 || a->rotary_dim > 4096 || a->rotary_dim % 2 != 0 || a->start < 0 || a->start > a->dim - a->rotary_dim)
     return DSA_STATUS_BAD_ARGUMENT;
   if (a->dtype < DSA_BF16 || a->dtype > DSA_FP32 || (a->layout != DSA_ROPE_INTERLEAVED && a->layout != DSA_ROPE_HALF))
     return DSA_STATUS_BAD_ARGUMENT;

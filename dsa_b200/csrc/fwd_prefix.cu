@@ -33,6 +33,8 @@
 // loads.
 #include <cuda.h>
 
+#include <atomic>
+
 #include "prefix.cuh"
 #include "umma_ptx.cuh"
 
@@ -758,8 +760,16 @@ bool encode(CUtensorMap* map, const void* ptr, long long rows, int blocks, int b
 }
 
 bool launch_config(cudaLaunchConfig_t* cfg, cudaLaunchAttribute* attr, unsigned ctas, cudaStream_t stream) {
-  if (cudaFuncSetAttribute(fwd_prefix_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes) != cudaSuccess)
-    return false;
+  // once per device: the attribute belongs to the device's context
+  static std::atomic<uint64_t> ready{0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if ((ready.load(std::memory_order_relaxed) & bit) == 0) {
+    if (cudaFuncSetAttribute(fwd_prefix_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes) != cudaSuccess)
+      return false;
+    ready.fetch_or(bit, std::memory_order_relaxed);
+  }
   attr->id = cudaLaunchAttributeClusterDimension;
   attr->val.clusterDim.x = 2;
   attr->val.clusterDim.y = 1;

@@ -21,7 +21,7 @@ namespace dsa {
 namespace {
 
 constexpr int kRoThreads = 256;
-constexpr int kRoTable = 2048;  // cosine pairs of a block
+constexpr int kRoTable = 2048;  // cosine pairs of a block (rotary_dim is at most 4096)
 
 // The two 16-bit numbers of a word, and back (one rounding each).
 template <typename T>
@@ -204,10 +204,10 @@ cudaError_t launch_v(const RotaryParams& p, cudaStream_t stream) {
   if (groups > p.heads) groups = p.heads;
   while (groups & (groups - 1)) groups += groups & -groups;  // a power of two: whole lines per warp
   if (groups > p.heads) groups = p.heads;
+  if (groups > 65535LL * kRoThreads / units) groups = 65535LL * kRoThreads / units;  // blocks of one token: grid.y
   const long long per_token = groups * units;
-  if (per_token > 0x7fffffffLL / 2) return cudaErrorInvalidConfiguration;
   int tpb = per_token < kRoThreads ? (int)(kRoThreads / per_token) : 1;
-  if (tpb > kRoTable / (p.rotary_dim / 2)) tpb = kRoTable / (p.rotary_dim / 2) > 0 ? kRoTable / (p.rotary_dim / 2) : 1;
+  if (tpb > kRoTable / (p.rotary_dim / 2)) tpb = kRoTable / (p.rotary_dim / 2);
   dim3 grid((unsigned)((p.tokens + tpb - 1) / tpb), 1, 1);
   if (tpb == 1) grid.y = (unsigned)((per_token + kRoThreads - 1) / kRoThreads);
   if (tpb < 1 || grid.y > 65535) return cudaErrorInvalidConfiguration;

@@ -69,20 +69,21 @@ def plan_pages(block_table, cached_lens, new_lens, free_blocks, free_count, bloc
             raise ValueError("block_table, lengths and free pages must be int32 and reset bool")
     if max(max_blocks, num_blocks) * block_size > 0x7fffffff or batch * max(queries, max_blocks) > 0x7fffffff:
         raise ValueError("a table, the page pool or the step holds more than 2^31 - 1 entries")
-    # separate tensors: a view costs more host time than an allocation
-    ints = {"dtype": torch.int32, "device": device}
-    positions, lengths = torch.empty((batch, queries), **ints), torch.empty((batch, queries), **ints)
-    slots, missing, work = torch.empty((batch, queries), **ints), torch.empty(1, **ints), torch.empty(4 * batch + 4, **ints)
+    # few allocations and views: they cost more host time than the kernels take
+    positions, lengths, slots = torch.empty((3, batch, queries), dtype=torch.int32, device=device).unbind(0)
+    words = 4 * batch + 4
     if inplace:
         table, lens, stack, count = block_table, cached_lens, free_blocks, free_count
+        work, missing = torch.empty(words + 1, dtype=torch.int32, device=device).split_with_sizes((words, 1))
     else:
-        table, lens = torch.empty_like(block_table), torch.empty_like(cached_lens)
-        stack, count = torch.empty_like(free_blocks), torch.empty_like(free_count)
+        table, stack = torch.empty_like(block_table), torch.empty_like(free_blocks)
+        work, missing, count, lens = torch.empty(words + 2 + batch, dtype=torch.int32, device=device).split_with_sizes(
+            (words, 1, 1, batch))
     api.enqueue("dsa_plan_pages", _native.PlanPagesArgs(
         block_table.data_ptr(), cached_lens.data_ptr(), new_lens.data_ptr(), free_blocks.data_ptr(),
         free_count.data_ptr(), None if reset is None else reset.data_ptr(), table.data_ptr(), lens.data_ptr(),
         positions.data_ptr(), lengths.data_ptr(), slots.data_ptr(), stack.data_ptr(), count.data_ptr(),
-        missing.data_ptr(), batch, queries, max_blocks, num_blocks, block_size, work.data_ptr(), 16 * batch + 16), index)
+        missing.data_ptr(), batch, queries, max_blocks, num_blocks, block_size, work.data_ptr(), 4 * words), index)
     return PagePlan(table, lens, positions, lengths, slots, stack, count, missing)
 
 

@@ -158,8 +158,8 @@ def rotary(x, positions, inv_freq, *, layout="interleaved", start=0, attention_f
     turned, dim = 2 * inv_freq.shape[0], shape[-1]
     if type(start) is not int or start < 0 or turned == 0 or start + turned > dim:
         raise ValueError("need 0 <= start and start + 2 * len(inv_freq) <= D")
-    if turned > 8192 or dim > 65536:
-        raise ValueError("at most 8192 turned elements of a row of at most 65536")
+    if turned > 4096 or dim > 65536:
+        raise ValueError("at most 4096 turned elements of a row of at most 65536")
     if x.stride(-1) != 1:
         raise ValueError("the last dimension of x must be contiguous")
     inverse = bool(inverse)

@@ -9,13 +9,12 @@ index row (dsa/api.py:76-132).
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _native, api
 
 WORKSPACE_BUDGET = 1 << 31  # bytes of FP32 partials per library call
+_AUTO = _native.Launch()  # family 0: the library's choice
 
 
 def forward_shared_prefix(q, prefix_kv, q_rope, prefix_k_rope, kv=None, k_rope=None, indices=None, *, prefix_len=None,
@@ -37,44 +36,43 @@ def forward_shared_prefix(q, prefix_kv, q_rope, prefix_k_rope, kv=None, k_rope=N
     and sum 0. Asynchronous on the current stream; partials are FP32, in
     pieces of whole queries that keep them under ``WORKSPACE_BUDGET`` bytes.
     """
-    if q.dim() != 4 or prefix_kv.dim() != 4:
+    shape = q.shape
+    if len(shape) != 4 or prefix_kv.dim() != 4:
         raise ValueError("q and prefix_kv must be 4-D tensors")
-    batch, queries, heads, width = q.shape
+    batch, queries, heads, width = shape
     prefix = prefix_kv.shape[1]
-    if (width != 512 or 0 in q.shape or prefix == 0 or q_rope.shape != (batch, queries, heads, 64)
+    if (width != 512 or 0 in shape or prefix == 0 or q_rope.shape != (batch, queries, heads, 64)
             or prefix_kv.shape != (1, prefix, 1, 512) or prefix_k_rope.shape != (1, prefix, 1, 64)):
         raise ValueError("need q[B,SQ,H,512], q_rope[B,SQ,H,64], prefix_kv[1,P,1,512], prefix_k_rope[1,P,1,64]")
     if heads % 16:
         raise ValueError("the head count must be a multiple of 16")
-    tensors = [q, q_rope, prefix_kv, prefix_k_rope]
+    halves, ints = [q, q_rope, prefix_kv, prefix_k_rope], []
     length = topk = 0
-    if kv is None and k_rope is None and indices is None:
-        pass
-    elif kv is None or k_rope is None or indices is None:
-        raise ValueError("kv, k_rope and indices go together")
-    else:
+    if kv is not None or k_rope is not None or indices is not None:
+        if kv is None or k_rope is None or indices is None:
+            raise ValueError("kv, k_rope and indices go together")
         if kv.dim() != 4 or indices.dim() != 4:
             raise ValueError("kv and indices must be 4-D tensors")
         length, topk = kv.shape[1], indices.shape[-1]
         if (kv.shape != (batch, length, 1, 512) or k_rope.shape != (batch, length, 1, 64)
                 or indices.shape != (batch, queries, 1, topk) or length == 0 or topk == 0):
             raise ValueError("need kv[B,L,1,512], k_rope[B,L,1,64], indices[B,SQ,1,K]")
-        if indices.dtype != torch.int32:
-            raise ValueError("indices must be int32")
-        tensors += [kv, k_rope, indices]
-    device, index = q.device, q.get_device()
+        halves += (kv, k_rope)
+        ints.append(indices)
     if prefix_len is not None:
-        if prefix_len.numel() != 1 or prefix_len.dtype != torch.int32:
+        if prefix_len.numel() != 1:
             raise ValueError("prefix_len must be an int32 tensor of one element")
-        tensors.append(prefix_len)
+        ints.append(prefix_len)
+    device, index = q.device, q.get_device()
     if device.type != api.DEVICE_TYPE:
         raise ValueError("all inputs must be contiguous and on the same CUDA device")
-    for t in tensors:
-        if t.get_device() != index or not t.is_contiguous():
-            raise ValueError("all inputs must be contiguous and on the same CUDA device")
-        if t.dtype != torch.bfloat16 and t is not indices and t is not prefix_len:
-            raise ValueError("q, q_rope, the prefix and kv/k_rope must be bfloat16")
-    scale_arg = api._check_scale(scale)
+    for tensors, dtype in ((halves, torch.bfloat16), (ints, torch.int32)):
+        for t in tensors:
+            if t.dtype != dtype:
+                raise ValueError("q, q_rope, the prefix and kv/k_rope must be bfloat16, indices and prefix_len int32")
+            if t.get_device() != index or not t.is_contiguous():
+                raise ValueError("all inputs must be contiguous and on the same CUDA device")
+    scale_arg = 0.0 if scale is None else api._check_scale(scale)
     if prefix > 1 << 30 or batch * queries > 0x7fffffff or batch * length > 0x7fffffff:
         raise ValueError("the prefix holds more than 2^30 rows, or the batch more than 2^31 - 1 queries or keys")
     output = torch.empty_like(q)
@@ -83,20 +81,20 @@ def forward_shared_prefix(q, prefix_kv, q_rope, prefix_k_rope, kv=None, k_rope=N
     lib = _native.load()
     px = _native.PrefixKv(prefix_kv.data_ptr(), prefix_k_rope.data_ptr(),
                           None if prefix_len is None else prefix_len.data_ptr(), prefix)
+    bases = [t.data_ptr() for t in (q, q_rope, output, maximum, denominator)]
+    own = (kv.data_ptr(), k_rope.data_ptr(), indices.data_ptr()) if topk else (None, None, None)
     status = api._status_word(device).data_ptr()
 
     def call(b0, b1, s0, s1):
         t0 = b0 * queries + s0
-        a = _native.FwdArgs()
-        a.q, a.q_rope = q.data_ptr() + t0 * heads * 1024, q_rope.data_ptr() + t0 * heads * 128
-        if topk:
-            a.kv, a.k_rope = kv.data_ptr() + b0 * length * 1024, k_rope.data_ptr() + b0 * length * 128
-            a.indices = indices.data_ptr() + t0 * topk * 4
-        a.output = output.data_ptr() + t0 * heads * 1024
-        a.softmax_max, a.softmax_sum = maximum.data_ptr() + t0 * heads * 4, denominator.data_ptr() + t0 * heads * 4
-        a.batch, a.queries, a.heads, a.length, a.topk = b1 - b0, s1 - s0, heads, length, topk
-        a.scale, a.status = scale_arg, status
-        need = int(lib.dsa_fwd_prefix_workspace_bytes(a, px))
+        rows = t0 * heads
+        q_at, qr_at, out_at, max_at, sum_at = (at + rows * n for at, n in zip(bases, (1024, 128, 1024, 4, 4)))
+        kv_at, kr_at, ids_at = own
+        if topk and t0:
+            kv_at, kr_at, ids_at = kv_at + b0 * length * 1024, kr_at + b0 * length * 128, ids_at + t0 * topk * 4
+        a = _native.FwdArgs(q_at, kv_at, qr_at, kr_at, ids_at, out_at, max_at, sum_at, b1 - b0, s1 - s0, heads, length,
+                            topk, _AUTO, None, 0, status, scale_arg)
+        need = lib.dsa_fwd_prefix_workspace_bytes(a, px)
         if need > WORKSPACE_BUDGET and (b1 - b0) * (s1 - s0) > 1:
             return False
         if need:

@@ -248,7 +248,7 @@ typedef struct dsa_rotary_args {
   int64_t batch, queries, heads, dim;
   int64_t x_stride[3], y_stride[3];  /* batch, query, head, in elements */
   int64_t position_stride[2];        /* batch, query */
-  int32_t rotary_dim, start;         /* rotary_dim even, at most 8192 */
+  int32_t rotary_dim, start;         /* rotary_dim even, at most 4096; dim at most 65536 */
   int32_t dtype;             /* dsa_dtype_t */
   int32_t positions64;
   int32_t layout;            /* dsa_rope_layout_t */

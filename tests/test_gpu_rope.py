@@ -48,7 +48,7 @@ def _make(shape, dtype, seed, far=100000):
 @pytest.mark.parametrize("shape,rotary_dim,start", [
     ((1, 1, 1, 64), 64, 0), ((3, 5, 7, 64), 64, 0), ((1, 9, 64, 128), 64, 0), ((2, 3, 16, 192), 64, 128),
     ((2, 129, 2, 96), 32, 32), ((2, 3, 5, 11), 6, 3), ((1, 1, 1, 2), 2, 0), ((2, 2, 3, 30), 30, 0), ((2, 7, 576), 64, 512),
-    ((1, 2, 300, 64), 64, 0), ((70, 130, 3, 72), 64, 8), ((1, 1, 1, 1024), 1024, 0), ((4, 40, 128, 24), 16, 8)])
+    ((1, 2, 300, 64), 64, 0), ((70, 130, 3, 72), 64, 8), ((1, 1, 1, 1024), 1024, 0), ((2, 3, 2, 4096), 4096, 0), ((1, 2, 3, 65536), 64, 65000), ((1, 1, 40000, 66), 66, 0), ((4, 40, 128, 24), 16, 8)])
 def test_rotary(cuda_lib, shape, rotary_dim, start, dtype, layout):
     x, pos = _make(shape, dtype, sum(shape))
     freq = dsa_b200.rotary_frequencies(rotary_dim, device="cuda")

@@ -107,6 +107,14 @@ def test_filled_part(cuda_lib, topk):
         _check(got, args, min(n, 700))
 
 
+def test_filled_part_without_partials(cuda_lib):
+    """Rows enough for the kernel to write the output itself (no split, no own keys)."""
+    args = _make(170, 1, 128, 130, 0, 0, seed=4)
+    args[1][0, 70:] = float("nan")
+    for n in (0, 1, 64, 70):
+        _check(dsa_b200.forward_shared_prefix(*args, prefix_len=torch.tensor([n], dtype=torch.int32, device="cuda")), args, n)
+
+
 def test_scale_and_repeat(cuda_lib):
     args = _make(4, 3, 64, 5000, 300, 200, seed=5)
     first = dsa_b200.forward_shared_prefix(*args, scale=0.11)

@@ -49,6 +49,8 @@ def test_rotary_refusals(monkeypatch):
         ((x, pos, t(16, dtype=torch.float64)), dict(start=33), "start"),
         ((x, pos, t(16, dtype=torch.float64)), dict(start=-1), "start"),
         ((x, pos, t(0, dtype=torch.float64)), {}, "start"),
+        ((t(2, 3, 4, 4098), pos, t(2049, dtype=torch.float64)), {}, "4096"),
+        ((t(2, 3, 65537), pos, freq), {}, "65536"),
         ((x, pos, freq), dict(layout="other"), "layout"),
         ((x, pos, freq), dict(attention_factor=float("nan")), "attention_factor"),
         ((t(2, 3, 64, 4).transpose(2, 3), pos, freq), {}, "last dimension"),
