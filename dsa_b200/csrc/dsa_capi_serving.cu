@@ -33,30 +33,36 @@ uint64_t align_up(uint64_t x) { return (x + kAlign - 1) / kAlign * kAlign; }
 // Launches of one shared-prefix call and its workspace.
 struct PrefixPlan {
   int64_t tokens, rows, row_tiles;
-  int split, own_split;  // own_split 0: no own keys
+  int group, split, own_split;  // own_split 0: no own keys
   bool direct;           // the prefix kernel writes the output
   uint64_t num, max, sum, own_num, own_max, own_sum, total;
 };
 
-// Key splits of the prefix: a cluster's time is its tiles plus a start of
-// about six (launch, TMEM, first loads), in waves of the resident clusters;
-// split partials cost a write and a read of 2 KB a row, about 5 TB/s (a tile
-// of 64 keys takes ~0.6 us).
-int prefix_split(int64_t row_tiles, int64_t keys, int clusters) {
-  const int64_t tiles = (keys + 63) / 64;
+// Row tiles per item (1 or 2) and key splits of the prefix: a cluster's time
+// is its tiles plus a start and an end of about twelve (launch, TMEM, Q, first
+// loads, stores), in waves of the resident clusters; split partials cost a write
+// and a read of 2 KB a row, about 5 TB/s, and the join ~0.3 us a part (96 rows
+// over 1000 keys: 8 splits 17.9 us, 16 splits 20.6). A tile of 64 keys takes a cluster of one row tile ~1,400
+// cycles and one of two ~1,200; the latter leaves half a cluster idle when the
+// row tiles are odd. Returns the estimated time.
+double prefix_split(int64_t row_tiles, int64_t keys, int group, int* split) {
+  int clusters = dsa::prefix_max_clusters(group);
+  if (clusters <= 0) clusters = 74 / group;
+  const int64_t tiles = (keys + 63) / 64, sets = (row_tiles + group - 1) / group;
+  const double tile_us = group == 1 ? 0.85 : 0.73;
   double best = 0;
-  int split = 1;
+  *split = 1;
   // more than four waves of items never pay
-  for (int s = 1; s <= 128 && s <= tiles && (s == 1 || row_tiles * s <= 4 * (int64_t)clusters); ++s) {
-    const int64_t waves = (row_tiles * s + clusters - 1) / clusters;
-    const double us = 0.6 * (double)waves * (double)((tiles + s - 1) / s + 6) +
-                      (s > 1 ? (double)row_tiles * s * 128 * 4096 / 5e6 : 0.0);
+  for (int s = 1; s <= 128 && s <= tiles && (s == 1 || sets * s <= 4 * (int64_t)clusters); ++s) {
+    const int64_t waves = (sets * s + clusters - 1) / clusters;
+    const double us = tile_us * (double)waves * (double)((tiles + s - 1) / s + 12) +
+                      (s > 1 ? 1.0 + 0.3 * s + (double)row_tiles * s * 128 * 4096 / 5e6 : 0.0);
     if (s == 1 || us < best) {
       best = us;
-      split = s;
+      *split = s;
     }
   }
-  return split;
+  return best;
 }
 
 bool plan_prefix(const dsa_fwd_args_t* a, const dsa_prefix_kv_t* px, PrefixPlan* plan) {
@@ -69,10 +75,11 @@ bool plan_prefix(const dsa_fwd_args_t* a, const dsa_prefix_kv_t* px, PrefixPlan*
   if (!product_ok(plan->tokens, a->heads, 1LL << 37)) return false;
   plan->rows = plan->tokens * a->heads;
   plan->row_tiles = (plan->rows + 127) / 128;
-  int clusters = dsa::prefix_max_clusters();
-  if (clusters <= 0) clusters = 74;
-  plan->split = prefix_split(plan->row_tiles, px->rows, clusters);
-  if (plan->row_tiles * plan->split > kMaxInt / 2) return false;
+  int split1 = 1, split2 = 1;
+  const double one = prefix_split(plan->row_tiles, px->rows, 1, &split1), two = prefix_split(plan->row_tiles, px->rows, 2, &split2);
+  plan->group = plan->row_tiles > 1 && two < one ? 2 : 1;
+  plan->split = plan->group == 2 ? split2 : split1;
+  if ((plan->row_tiles + 1) * plan->split > kMaxInt / 2) return false;
   plan->own_split = 0;
   if (own) {
     // own keys: one wave of the pair (H = 128) or stream family's CTAs, two
@@ -256,6 +263,7 @@ int dsa_sparse_mla_fwd_prefix(const dsa_fwd_args_t* a, const dsa_prefix_kv_t* px
   p.rows = plan.rows;
   p.keys = (int)px->rows;
   p.split = plan.split;
+  p.group = plan.group;
   p.scale_div = f.scale_div;
   p.scale_log2 = f.scale_log2;
   int st = launch_status(dsa::launch_fwd_prefix(p, px->kv, px->k_rope, s));

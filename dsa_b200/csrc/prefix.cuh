@@ -18,6 +18,7 @@ struct PrefixParams {
   int32_t* status;
   long long rows;               // queries x heads, even
   int keys, split;
+  int group;                    // row tiles of an item and CTAs of an MMA pair: 1 or 2
   float scale_div, scale_log2;
 };
 
@@ -35,8 +36,9 @@ struct JoinParams {
   int heads, split, own_split;
 };
 
-// Clusters of the prefix kernel that are resident at once (-1 on error).
-int prefix_max_clusters();
+// Clusters of the prefix kernel with `group` row tiles that are resident at
+// once (-1 on error).
+int prefix_max_clusters(int group);
 cudaError_t launch_fwd_prefix(const PrefixParams& p, const void* kv, const void* k_rope, cudaStream_t stream);
 cudaError_t launch_prefix_join(const JoinParams& p, cudaStream_t stream);
 

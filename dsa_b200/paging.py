@@ -46,38 +46,39 @@ def plan_pages(block_table, cached_lens, new_lens, free_blocks, free_count, bloc
     ``cached_lens`` (to ``seq_lens``), ``free_blocks`` and ``free_count``; the
     call is asynchronous, allocates through torch and can be captured.
     """
-    if block_table.dim() != 2 or type(block_size) is not int or type(queries) is not int or block_size <= 0 or queries <= 0:
+    if type(block_size) is not int or type(queries) is not int or block_size <= 0 or queries <= 0 or block_table.dim() != 2:
         raise ValueError("block_table must be 2-D, block_size and queries positive ints")
     batch, max_blocks = block_table.shape
-    num_blocks = free_blocks.shape[0] if free_blocks.dim() == 1 else 0
+    num_blocks = free_blocks.numel()
     rows = cached_lens.shape
-    if (not batch or not max_blocks or not num_blocks or rows != (batch,) or new_lens.shape != rows
-            or free_count.numel() != 1 or (reset is not None and reset.shape != rows)):
+    if (not batch or not max_blocks or not num_blocks or free_blocks.dim() != 1 or rows != (batch,)
+            or new_lens.shape != rows or free_count.numel() != 1 or (reset is not None and reset.shape != rows)):
         raise ValueError("need block_table[B,MB], cached_lens[B], new_lens[B], free_blocks[NB], free_count[1], reset[B]")
-    device, index = block_table.device, block_table.get_device()
+    device, index, int32 = block_table.device, block_table.get_device(), torch.int32
     if device.type != api.DEVICE_TYPE:
         raise ValueError("all inputs must be contiguous and on the same CUDA device")
     for t in (block_table, cached_lens, new_lens, free_blocks, free_count):
+        if t.dtype is not int32:
+            raise ValueError("block_table, lengths and free pages must be int32 and reset bool")
         if t.get_device() != index or not t.is_contiguous():
             raise ValueError("all inputs must be contiguous and on the same CUDA device")
-        if t.dtype != torch.int32:
-            raise ValueError("block_table, lengths and free pages must be int32 and reset bool")
     if reset is not None:
+        if reset.dtype is not torch.bool:
+            raise ValueError("block_table, lengths and free pages must be int32 and reset bool")
         if reset.get_device() != index or not reset.is_contiguous():
             raise ValueError("all inputs must be contiguous and on the same CUDA device")
-        if reset.dtype != torch.bool:
-            raise ValueError("block_table, lengths and free pages must be int32 and reset bool")
-    if max(max_blocks, num_blocks) * block_size > 0x7fffffff or batch * max(queries, max_blocks) > 0x7fffffff:
+    if (max_blocks * block_size > 0x7fffffff or num_blocks * block_size > 0x7fffffff or batch * queries > 0x7fffffff
+            or batch * max_blocks > 0x7fffffff):
         raise ValueError("a table, the page pool or the step holds more than 2^31 - 1 entries")
     # few allocations and views: they cost more host time than the kernels take
-    positions, lengths, slots = torch.empty((3, batch, queries), dtype=torch.int32, device=device).unbind(0)
+    positions, lengths, slots = torch.empty((3, batch, queries), dtype=int32, device=device).unbind(0)
     words = 4 * batch + 4
     if inplace:
         table, lens, stack, count = block_table, cached_lens, free_blocks, free_count
-        work, missing = torch.empty(words + 1, dtype=torch.int32, device=device).split_with_sizes((words, 1))
+        work, missing = torch.empty(words + 1, dtype=int32, device=device).split_with_sizes((words, 1))
     else:
         table, stack = torch.empty_like(block_table), torch.empty_like(free_blocks)
-        work, missing, count, lens = torch.empty(words + 2 + batch, dtype=torch.int32, device=device).split_with_sizes(
+        work, missing, count, lens = torch.empty(words + 2 + batch, dtype=int32, device=device).split_with_sizes(
             (words, 1, 1, batch))
     api.enqueue("dsa_plan_pages", _native.PlanPagesArgs(
         block_table.data_ptr(), cached_lens.data_ptr(), new_lens.data_ptr(), free_blocks.data_ptr(),
@@ -87,46 +88,48 @@ def plan_pages(block_table, cached_lens, new_lens, free_blocks, free_count, bloc
     return PagePlan(table, lens, positions, lengths, slots, stack, count, missing)
 
 
-def _append(kv, k_rope, slots, latent, rope, fp8, positions, inv_freq, layout, attention_factor):
-    """Checks and launch; the caches are ``latent`` and ``rope``, or ``fp8``."""
-    shape, index = kv.shape, kv.get_device()
-    if len(shape) != 4 or shape[2:] != (1, 512) or 0 in shape or k_rope.shape != (*shape[:3], 64):
+def _append(kv, k_rope, slots, latent, rope, fp8, rows, positions, inv_freq, layout, attention_factor):
+    """Checks and launch; the caches (``rows`` rows, shapes and types checked) are ``latent`` and ``rope``, or ``fp8``."""
+    shape, index, bf16, int32 = kv.shape, kv.get_device(), torch.bfloat16, torch.int32
+    if len(shape) != 4 or shape[2] != 1 or shape[3] != 512 or not shape[0] or not shape[1]:
         raise ValueError("need kv[B,S,1,512] and k_rope[B,S,1,64]")
-    lead = shape[:2]
-    if slots.shape != lead or slots.dtype != torch.int32:
+    batch, queries, _, _ = shape
+    if k_rope.shape != (batch, queries, 1, 64):
+        raise ValueError("need kv[B,S,1,512] and k_rope[B,S,1,64]")
+    lead = slots.shape
+    if lead != (batch, queries) or slots.dtype is not int32:
         raise ValueError("slots must be int32 [B,S]")
-    if kv.dtype != torch.bfloat16 or k_rope.dtype != torch.bfloat16:
+    if kv.dtype is not bf16 or k_rope.dtype is not bf16:
         raise ValueError("kv and k_rope must be bfloat16")
-    (kv0, kv1, _, kv3), (kr0, kr1, _, kr3) = kv.stride(), k_rope.stride()
+    kv0, kv1, _, kv3 = kv.stride()
+    kr0, kr1, _, kr3 = k_rope.stride()
     if kv3 != 1 or kr3 != 1:
         raise ValueError("the last dimension of kv and k_rope must be contiguous")
-    if kv.device.type != api.DEVICE_TYPE or k_rope.get_device() != index or slots.get_device() != index:
+    first = latent if fp8 is None else fp8
+    if (kv.device.type != api.DEVICE_TYPE or k_rope.get_device() != index or slots.get_device() != index
+            or first.get_device() != index or (rope is not None and rope.get_device() != index)):
         raise ValueError("all inputs must be on the same CUDA device")
-    if not slots.is_contiguous():
+    if not slots.is_contiguous() or not first.is_contiguous() or (rope is not None and not rope.is_contiguous()):
         raise ValueError("slots and the cache must be contiguous")
-    for cache in (latent, rope) if fp8 is None else (fp8,):
-        if cache.get_device() != index:
-            raise ValueError("all inputs must be on the same CUDA device")
-        if not cache.is_contiguous():
-            raise ValueError("slots and the cache must be contiguous")
-        rows = cache.shape[0] * cache.shape[1]
-    if (positions is None) != (inv_freq is None):
-        raise ValueError("positions and inv_freq go together")
-    if inv_freq is not None:
+    if inv_freq is not None and positions is not None:
         number = _check_rope(positions, inv_freq, layout, attention_factor, lead, index)
-        if positions.dtype != torch.int32 or not positions.is_contiguous() or inv_freq.shape[0] != 32:
+        if positions.dtype is not int32 or not positions.is_contiguous() or inv_freq.shape[0] != 32:
             raise ValueError("positions must be contiguous int32 [B,S] and inv_freq have 32 entries")
+        pos_at, freq_at = positions.data_ptr(), inv_freq.data_ptr()
+    elif inv_freq is not None or positions is not None:
+        raise ValueError("positions and inv_freq go together")
     elif layout in _native.ROPE_LAYOUTS:
-        number, attention_factor = 0, 1.0
+        number, attention_factor, pos_at, freq_at = 0, 1.0, None, None
     else:
         raise ValueError("layout must be 'interleaved' or 'half'")
-    batch, queries = lead
     if rows > 0x7fffffff or batch * queries > 0x7fffffff:
         raise ValueError("the cache or the step holds more than 2^31 - 1 rows")
+    if fp8 is None:
+        caches = first.data_ptr(), rope.data_ptr(), None
+    else:
+        caches = None, None, first.data_ptr()
     api.enqueue("dsa_append_kv", _native.AppendKvArgs(
-        kv.data_ptr(), k_rope.data_ptr(), slots.data_ptr(), None if positions is None else positions.data_ptr(),
-        None if inv_freq is None else inv_freq.data_ptr(), None if latent is None else latent.data_ptr(),
-        None if rope is None else rope.data_ptr(), None if fp8 is None else fp8.data_ptr(), batch, queries, rows,
+        kv.data_ptr(), k_rope.data_ptr(), slots.data_ptr(), pos_at, freq_at, *caches, batch, queries, rows,
         kv0, kv1, kr0, kr1, number, attention_factor), index)
 
 
@@ -144,12 +147,16 @@ def append_kv(kv, k_rope, slots, kv_cache, k_rope_cache, *, positions=None, inv_
     ``[B, S]``) and ``inv_freq`` (FP64 ``[32]``) ``k_rope`` is turned first, as
     by ``rotary``; without them it is stored as given.
     """
-    if (kv_cache.dim() != 4 or k_rope_cache.dim() != 4 or kv_cache.shape[2:] != (1, 512) or 0 in kv_cache.shape
-            or k_rope_cache.shape != (*kv_cache.shape[:3], 64)):
+    shape = kv_cache.shape
+    if len(shape) != 4 or shape[2] != 1 or shape[3] != 512 or not shape[0] or not shape[1]:
         raise ValueError("need kv_cache[NB,BS,1,512] and k_rope_cache[NB,BS,1,64]")
-    if kv_cache.dtype != torch.bfloat16 or k_rope_cache.dtype != torch.bfloat16:
+    blocks, block_size, _, _ = shape
+    if k_rope_cache.shape != (blocks, block_size, 1, 64):
+        raise ValueError("need kv_cache[NB,BS,1,512] and k_rope_cache[NB,BS,1,64]")
+    if kv_cache.dtype is not torch.bfloat16 or k_rope_cache.dtype is not torch.bfloat16:
         raise ValueError("the caches must be bfloat16")
-    _append(kv, k_rope, slots, kv_cache, k_rope_cache, None, positions, inv_freq, layout, attention_factor)
+    _append(kv, k_rope, slots, kv_cache, k_rope_cache, None, blocks * block_size, positions, inv_freq, layout,
+            attention_factor)
 
 
 def append_kv_fp8(kv, k_rope, slots, cache, *, positions=None, inv_freq=None, layout="interleaved",
@@ -163,8 +170,9 @@ def append_kv_fp8(kv, k_rope, slots, cache, *, positions=None, inv_freq=None, la
     ``amax / 448`` is torch's product with the rounded 1 / 448, so its scales
     may be one FP32 step away.)
     """
-    if cache.dim() != 4 or cache.shape[2:] != (1, _native.FP8_ROW_BYTES) or 0 in cache.shape:
+    shape = cache.shape
+    if len(shape) != 4 or shape[2] != 1 or shape[3] != _native.FP8_ROW_BYTES or not shape[0] or not shape[1]:
         raise ValueError("need cache[NB,BS,1,656]")
-    if cache.dtype != torch.uint8:
+    if cache.dtype is not torch.uint8:
         raise ValueError("the FP8 cache must be uint8")
-    _append(kv, k_rope, slots, None, None, cache, positions, inv_freq, layout, attention_factor)
+    _append(kv, k_rope, slots, None, None, cache, shape[0] * shape[1], positions, inv_freq, layout, attention_factor)

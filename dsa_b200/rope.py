@@ -78,7 +78,7 @@ def _check_rope(positions, inv_freq, layout, attention_factor, lead, index):
         raise ValueError("attention_factor must be a finite number")
     if positions.shape != lead or positions.dtype not in _POSITIONS:
         raise ValueError("positions must be int32 or int64 and have one entry per token")
-    if inv_freq.dim() != 1 or inv_freq.dtype != torch.float64 or not inv_freq.is_contiguous():
+    if inv_freq.dtype is not torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
         raise ValueError("inv_freq must be a contiguous 1-D float64 tensor (FP32 frequencies lose far positions)")
     if positions.get_device() != index or inv_freq.get_device() != index:
         raise ValueError("all inputs must be on the same CUDA device")
@@ -88,18 +88,20 @@ def _check_rope(positions, inv_freq, layout, attention_factor, lead, index):
 
 
 def _launch(x, positions, inv_freq, out, number, start, factor, inverse):
-    shape, (p0, p1) = x.shape, positions.stride()
-    if len(shape) == 3:
-        (batch, queries, dim), heads = shape, 1
-        (x0, x1, _), (y0, y1, _) = x.stride(), out.stride()
-        x2 = y2 = 0
+    p0, p1 = positions.stride()
+    if x.dim() == 4:
+        batch, queries, heads, dim = x.shape
+        x0, x1, x2, _ = x.stride()
+        y0, y1, y2, _ = out.stride()
     else:
-        batch, queries, heads, dim = shape
-        (x0, x1, x2, _), (y0, y1, y2, _) = x.stride(), out.stride()
+        batch, queries, dim = x.shape
+        x0, x1, _ = x.stride()
+        y0, y1, _ = out.stride()
+        heads, x2, y2 = 1, 0, 0
     api.enqueue("dsa_rotary", _native.RotaryArgs(
         x.data_ptr(), out.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(), batch, queries, heads, dim,
         x0, x1, x2, y0, y1, y2, p0, p1, 2 * inv_freq.shape[0], start, _DTYPES[x.dtype],
-        positions.dtype == torch.int64, number, inverse, factor), x.get_device())
+        positions.dtype is torch.int64, number, inverse, factor), x.get_device())
     return out
 
 

@@ -81,6 +81,13 @@ def test_parity(cuda_lib, batch, queries, heads, prefix, length, topk, gain):
     _check(dsa_b200.forward_shared_prefix(*args), args, prefix)
 
 
+@pytest.mark.parametrize("rows", [1, 2, 3, 160])  # row tiles: one MMA CTA, a pair, a pair and a half, without a split
+@pytest.mark.parametrize("prefix", [1, 63, 64, 65, 128, 129, 300, 1100])
+def test_lengths(cuda_lib, rows, prefix):
+    args = _make(rows, 1, 128, prefix, 0, 0, seed=prefix)
+    _check(dsa_b200.forward_shared_prefix(*args), args, prefix)
+
+
 @pytest.mark.parametrize("topk", [0, 40])
 def test_filled_part(cuda_lib, topk):
     """A buffer filled in part: lengths on every side of a tile's end, NaN and infinities behind the last key; one captured
