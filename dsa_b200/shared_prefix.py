@@ -46,8 +46,10 @@ def forward_shared_prefix(q, prefix_kv, q_rope, prefix_k_rope, kv=None, k_rope=N
         raise ValueError("need q[B,SQ,H,512], q_rope[B,SQ,H,64], prefix_kv[1,P,1,512], prefix_k_rope[1,P,1,64]")
     if heads % 16:
         raise ValueError("the head count must be a multiple of 16")
-    halves, ints = [q, q_rope, prefix_kv, prefix_k_rope], []
-    length = topk = 0
+    device, index, bf16, length, topk = q.device, q.get_device(), torch.bfloat16, 0, 0
+    if device.type != api.DEVICE_TYPE:
+        raise ValueError("all inputs must be contiguous and on the same CUDA device")
+    tensors = (q, q_rope, prefix_kv, prefix_k_rope)
     if kv is not None or k_rope is not None or indices is not None:
         if kv is None or k_rope is None or indices is None:
             raise ValueError("kv, k_rope and indices go together")
@@ -57,61 +59,70 @@ def forward_shared_prefix(q, prefix_kv, q_rope, prefix_k_rope, kv=None, k_rope=N
         if (kv.shape != (batch, length, 1, 512) or k_rope.shape != (batch, length, 1, 64)
                 or indices.shape != (batch, queries, 1, topk) or length == 0 or topk == 0):
             raise ValueError("need kv[B,L,1,512], k_rope[B,L,1,64], indices[B,SQ,1,K]")
-        halves += (kv, k_rope)
-        ints.append(indices)
-    if prefix_len is not None:
-        if prefix_len.numel() != 1:
-            raise ValueError("prefix_len must be an int32 tensor of one element")
-        ints.append(prefix_len)
-    device, index = q.device, q.get_device()
-    if device.type != api.DEVICE_TYPE:
-        raise ValueError("all inputs must be contiguous and on the same CUDA device")
-    for tensors, dtype in ((halves, torch.bfloat16), (ints, torch.int32)):
-        for t in tensors:
-            if t.dtype != dtype:
-                raise ValueError("q, q_rope, the prefix and kv/k_rope must be bfloat16, indices and prefix_len int32")
-            if t.get_device() != index or not t.is_contiguous():
-                raise ValueError("all inputs must be contiguous and on the same CUDA device")
+        tensors = (q, q_rope, prefix_kv, prefix_k_rope, kv, k_rope)
+    for t in tensors:
+        if t.dtype is not bf16:
+            raise ValueError("q, q_rope, the prefix and kv/k_rope must be bfloat16, indices and prefix_len int32")
+        if t.get_device() != index or not t.is_contiguous():
+            raise ValueError("all inputs must be contiguous and on the same CUDA device")
+    if prefix_len is not None and prefix_len.numel() != 1:
+        raise ValueError("prefix_len must be an int32 tensor of one element")
+    for t in (indices, prefix_len):
+        if t is None:
+            continue
+        if t.dtype is not torch.int32:
+            raise ValueError("q, q_rope, the prefix and kv/k_rope must be bfloat16, indices and prefix_len int32")
+        if t.get_device() != index or not t.is_contiguous():
+            raise ValueError("all inputs must be contiguous and on the same CUDA device")
     scale_arg = 0.0 if scale is None else api._check_scale(scale)
     if prefix > 1 << 30 or batch * queries > 0x7fffffff or batch * length > 0x7fffffff:
         raise ValueError("the prefix holds more than 2^30 rows, or the batch more than 2^31 - 1 queries or keys")
     output = torch.empty_like(q)
     maximum = torch.empty((batch, 1, queries, heads), device=device, dtype=torch.float32)
     denominator = torch.empty_like(maximum)
-    lib = _native.load()
     px = _native.PrefixKv(prefix_kv.data_ptr(), prefix_k_rope.data_ptr(),
                           None if prefix_len is None else prefix_len.data_ptr(), prefix)
-    bases = [t.data_ptr() for t in (q, q_rope, output, maximum, denominator)]
-    own = (kv.data_ptr(), k_rope.data_ptr(), indices.data_ptr()) if topk else (None, None, None)
-    status = api._status_word(device).data_ptr()
-
-    def call(b0, b1, s0, s1):
-        t0 = b0 * queries + s0
-        rows = t0 * heads
-        q_at, qr_at, out_at, max_at, sum_at = (at + rows * n for at, n in zip(bases, (1024, 128, 1024, 4, 4)))
-        kv_at, kr_at, ids_at = own
-        if topk and t0:
-            kv_at, kr_at, ids_at = kv_at + b0 * length * 1024, kr_at + b0 * length * 128, ids_at + t0 * topk * 4
-        a = _native.FwdArgs(q_at, kv_at, qr_at, kr_at, ids_at, out_at, max_at, sum_at, b1 - b0, s1 - s0, heads, length,
-                            topk, _AUTO, None, 0, status, scale_arg)
-        need = lib.dsa_fwd_prefix_workspace_bytes(a, px)
-        if need > WORKSPACE_BUDGET and (b1 - b0) * (s1 - s0) > 1:
-            return False
-        if need:
-            workspace = torch.empty(need, dtype=torch.uint8, device=device)
-            a.workspace, a.workspace_bytes = workspace.data_ptr(), need
-        api.enqueue("dsa_sparse_mla_fwd_prefix", a, index, px)
-        return True
-
-    pieces = [(0, batch, 0, queries)]
-    while pieces:  # halves of what does not fit, in order
-        b0, b1, s0, s1 = pieces.pop()
-        if call(b0, b1, s0, s1):
-            continue
-        if b1 - b0 > 1:
-            mid = (b0 + b1) // 2
-            pieces += [(mid, b1, s0, s1), (b0, mid, s0, s1)]
-        else:
-            mid = (s0 + s1) // 2
-            pieces += [(b0, b1, mid, s1), (b0, b1, s0, mid)]
+    args = _native.FwdArgs(
+        q.data_ptr(), kv.data_ptr() if topk else None, q_rope.data_ptr(), k_rope.data_ptr() if topk else None,
+        indices.data_ptr() if topk else None, output.data_ptr(), maximum.data_ptr(), denominator.data_ptr(), batch, queries,
+        heads, length, topk, _AUTO, None, 0, api._status_word(device).data_ptr(), scale_arg)
+    if not _enqueue(args, px, device, index):
+        # halves of what does not fit the workspace budget, in order: batch rows, then queries of one row
+        pieces = [(0, batch, 0, queries)]
+        while pieces:
+            b0, b1, s0, s1 = pieces.pop()
+            if _enqueue(_piece(args, b0, b1, s0, s1), px, device, index):
+                continue
+            if b1 - b0 > 1:
+                mid = (b0 + b1) // 2
+                pieces += [(mid, b1, s0, s1), (b0, mid, s0, s1)]
+            else:
+                mid = (s0 + s1) // 2
+                pieces += [(b0, b1, mid, s1), (b0, b1, s0, mid)]
     return output, maximum, denominator
+
+
+def _enqueue(args, px, device, index):
+    """Launch the call of ``args`` unless it takes more workspace than the budget and can be cut."""
+    need = _native.load().dsa_fwd_prefix_workspace_bytes(args, px)
+    if need:
+        if need > WORKSPACE_BUDGET and args.batch * args.queries > 1:
+            return False
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+        args.workspace, args.workspace_bytes = workspace.data_ptr(), need
+    api.enqueue("dsa_sparse_mla_fwd_prefix", args, index, px)
+    return True
+
+
+def _piece(args, b0, b1, s0, s1):
+    """The arguments for batch rows ``[b0, b1)`` and queries ``[s0, s1)`` (all of them when there are several rows)."""
+    t0 = b0 * args.queries + s0
+    rows = t0 * args.heads
+    piece = _native.FwdArgs.from_buffer_copy(args)
+    piece.q, piece.q_rope, piece.output = args.q + rows * 1024, args.q_rope + rows * 128, args.output + rows * 1024
+    piece.softmax_max, piece.softmax_sum = args.softmax_max + rows * 4, args.softmax_sum + rows * 4
+    if args.topk:
+        piece.kv, piece.k_rope = args.kv + b0 * args.length * 1024, args.k_rope + b0 * args.length * 128
+        piece.indices = args.indices + t0 * args.topk * 4
+    piece.batch, piece.queries = b1 - b0, s1 - s0
+    return piece
