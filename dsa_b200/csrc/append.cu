@@ -85,10 +85,10 @@ __device__ __forceinline__ void write_row(const AppendParams& p, long long slot,
     const float scale = amax > 0.f ? __fdiv_rn(amax, 448.f) : 1.f;
     // kv / scale, correctly rounded: with the correctly rounded reciprocal one
     // Newton step on the quotient's exact remainder gives it (Markstein, 1990)
-    // while nothing leaves the normal range; 16 divisions would cost a lane
-    // more than all the rest.
+    // while nothing leaves the normal range (a zero keeps its sign by hand);
+    // 16 divisions would cost a lane more than all the rest.
     uint32_t q[4];
-    if (scale >= 0x1p-60f && scale <= 0x1p60f) {
+    if (top < 0x7f80u && scale >= 0x1p-60f && scale <= 0x1p60f) {  // every value finite
       const float inv = __frcp_rn(scale);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -97,7 +97,7 @@ __device__ __forceinline__ void write_row(const AppendParams& p, long long slot,
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float y = __fmul_rn(x[i], inv);
-          x[i] = __fmaf_rn(__fmaf_rn(-y, scale, x[i]), inv, y);
+          x[i] = copysignf(__fmaf_rn(__fmaf_rn(-y, scale, x[i]), inv, y), y);
         }
         q[k] = pack_e4m3(x);
       }

@@ -68,7 +68,7 @@ double prefix_split(int64_t row_tiles, int64_t keys, int group, int* split) {
 bool plan_prefix(const dsa_fwd_args_t* a, const dsa_prefix_kv_t* px, PrefixPlan* plan) {
   if (a == nullptr || px == nullptr || a->launch.family != DSA_FAMILY_AUTO) return false;
   if (!product_ok(a->batch, a->queries) || a->heads <= 0 || a->heads > 65536 || a->heads % 16 != 0) return false;
-  if (px->rows <= 0 || px->rows > (1LL << 30)) return false;
+  if (px->rows <= 0 || px->rows > (1LL << 26)) return false;
   const bool own = a->topk > 0;
   if (a->topk < 0 || a->topk > kMaxInt || (own && (!product_ok(a->batch, a->length)))) return false;
   plan->tokens = a->batch * a->queries;

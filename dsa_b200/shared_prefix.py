@@ -75,8 +75,8 @@ def forward_shared_prefix(q, prefix_kv, q_rope, prefix_k_rope, kv=None, k_rope=N
         if t.get_device() != index or not t.is_contiguous():
             raise ValueError("all inputs must be contiguous and on the same CUDA device")
     scale_arg = 0.0 if scale is None else api._check_scale(scale)
-    if prefix > 1 << 30 or batch * queries > 0x7fffffff or batch * length > 0x7fffffff:
-        raise ValueError("the prefix holds more than 2^30 rows, or the batch more than 2^31 - 1 queries or keys")
+    if prefix > 1 << 26 or batch * queries > 0x7fffffff or batch * length > 0x7fffffff:
+        raise ValueError("the prefix holds more than 2^26 rows, or the batch more than 2^31 - 1 queries or keys")
     output = torch.empty_like(q)
     maximum = torch.empty((batch, 1, queries, heads), device=device, dtype=torch.float32)
     denominator = torch.empty_like(maximum)

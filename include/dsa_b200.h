@@ -335,7 +335,7 @@ typedef struct dsa_prefix_kv {
   const void* kv;          /* BF16 [rows, 512] */
   const void* k_rope;      /* BF16 [rows, 64] */
   const int32_t* length;   /* device INT32 [1]: the first length rows are keys (clamped to [0, rows]); NULL: all */
-  int64_t rows;
+  int64_t rows;            /* at most 2^26 (an item walks its split within the 2 s bound of the device-side waits) */
 } dsa_prefix_kv_t;
 
 /* Workspace bytes of dsa_sparse_mla_fwd_prefix; 0 for invalid arguments, and

@@ -192,6 +192,60 @@ def test_append_special_values(cuda_lib):
         assert torch.equal(torch.isnan(g), torch.isnan(w)) and torch.equal(g.nan_to_num(7.0), w.nan_to_num(7.0)), lo
 
 
+def test_append_signed_zeros_and_mixed_blocks(cuda_lib):
+    """Bit for bit the host writer's rows: zeros of both signs, values that round to them, and blocks that hold a NaN next
+    to infinities and the largest numbers (scale 1: those saturate)."""
+    kv, kr = _tokens(1, 4, 9)
+    kv[0, 0, 0, ::2] = -0.0
+    kv[0, 0, 0, 128:256] = -0.0
+    kv[0, 1] *= 2.0 ** torch.randint(-40, 2, (512,), device="cuda").float()
+    kv[0, 2, 0, 7], kv[0, 2, 0, 8], kv[0, 2, 0, 9], kv[0, 2, 0, 10] = float("nan"), float("inf"), float("-inf"), 3e38
+    slots = torch.arange(4, dtype=torch.int32, device="cuda").reshape(1, 4)
+    cache = torch.zeros((1, 4, 1, 656), dtype=torch.uint8, device="cuda")
+    dsa_b200.append_kv_fp8(kv, kr, slots, cache)
+    want = dsa_b200.quantize_kv_fp8(kv.cpu(), kr.cpu()).cuda()
+    nan = torch.isnan(want[..., :512].contiguous().view(torch.float8_e4m3fn).float())
+    assert torch.equal(torch.isnan(cache[..., :512].contiguous().view(torch.float8_e4m3fn).float()), nan)
+    assert torch.equal(cache[..., :512][~nan], want[..., :512][~nan]) and torch.equal(cache[..., 512:], want[..., 512:])
+
+
+def test_append_far_rows(cuda_lib):
+    """Rows behind 2^31 elements of the BF16 cache and 2^31 bytes of the FP8 cache; the rows around them stay."""
+    kv, kr = _tokens(1, 2, 10)
+    rows = (1 << 22) + 100
+    slots = torch.tensor([[rows - 1, rows - 3]], dtype=torch.int32, device="cuda")
+    pool = torch.zeros((rows, 1, 1, 512), dtype=torch.bfloat16, device="cuda")
+    rope = torch.zeros((rows, 1, 1, 64), dtype=torch.bfloat16, device="cuda")
+    dsa_b200.append_kv(kv, kr, slots, pool, rope)
+    assert torch.equal(pool[-1], kv[0, :1]) and torch.equal(pool[-3], kv[0, 1:]) and torch.equal(rope[-3], kr[0, 1:])
+    assert not bool(pool[-2].any()) and not bool(pool[:8].any())
+    del pool
+    cache = torch.zeros((rows, 1, 1, 656), dtype=torch.uint8, device="cuda")
+    dsa_b200.append_kv_fp8(kv, kr, slots, cache)
+    want = dsa_b200.quantize_kv_fp8(kv.cpu(), kr.cpu()).cuda()
+    assert torch.equal(cache[-1], want[0, :1]) and torch.equal(cache[-3], want[0, 1:]) and not bool(cache[-2].any())
+
+
+def test_captured_append_with_new_slots(cuda_lib):
+    kv, kr = _tokens(3, 1, 11)
+    slots, pos = torch.full((3, 1), -1, dtype=torch.int32, device="cuda"), torch.zeros((3, 1), dtype=torch.int32, device="cuda")
+    freq = dsa_b200.rotary_frequencies(64, device="cuda")
+    pools = [torch.zeros((40, 1, 1, n), dtype=torch.bfloat16, device="cuda") for n in (512, 64)]
+    dsa_b200.append_kv(kv, kr, slots, *pools, positions=pos, inv_freq=freq)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        dsa_b200.append_kv(kv, kr, slots, *pools, positions=pos, inv_freq=freq)
+    want = [t.clone() for t in pools]
+    for k in range(4):
+        slots.copy_(torch.tensor([[k], [20 + k], [-1]]))
+        pos.fill_(1000 * k)
+        kv.neg_()
+        graph.replay()
+        want[0][[k, 20 + k], 0] = kv[:2, 0]
+        want[1][[k, 20 + k], 0] = dsa_b200.rotary(kr, pos, freq)[:2, 0]
+        assert torch.equal(pools[0], want[0]) and torch.equal(pools[1], want[1])
+
+
 def test_append_without_alignment(cuda_lib):
     """kv rows that start on no 16-byte boundary."""
     kv, kr = _tokens(2, 5, 8)

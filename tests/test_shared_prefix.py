@@ -32,6 +32,7 @@ def test_refusals(monkeypatch):
         ((q, pk.half(), qr, pr), {}, "bfloat16"), ((q, pk, qr, pr, kv.float(), kr, ids), {}, "bfloat16"),
         ((t(3, 2, 16, 512).transpose(0, 1), pk, qr, pr), {}, "contiguous"),
         ((q, pk, qr, pr), dict(scale=0.75), "scale"),
+        ((q, t(1, (1 << 26) + 1, 1, 512), qr, t(1, (1 << 26) + 1, 1, 64)), {}, "2\\^26"),
     ]:
         with pytest.raises(ValueError, match=why):
             dsa_b200.forward_shared_prefix(*args, **kw)
