@@ -303,7 +303,7 @@ int dsa_sparse_mla_fwd_prefix(const dsa_fwd_args_t* a, const dsa_prefix_kv_t* px
     f.keys_per_tile = 32;
     f.heads_per_cta = a->heads == 128 ? 128 : 16;
     f.beside_previous = 1;  // fills the SMs that the prefix kernel leaves
-    st = launch_status(a->heads == 128 ? dsa::launch_fwd_pair(f, s) : dsa::launch_fwd_stream(f, s, false));
+    st = launch_status(a->heads == 128 ? dsa::launch_fwd_pair(f, s) : dsa::launch_fwd_stream(f, s));
     if (st != DSA_STATUS_OK) return st;
   }
   return launch_status(dsa::launch_prefix_join(j, s));

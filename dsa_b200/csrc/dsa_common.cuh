@@ -48,8 +48,7 @@ struct FwdParams {
   __nv_bfloat16* out;     // split == 1
   float* out_max;         // split == 1
   float* out_sum;         // split == 1
-  float* part_num;        // split > 1: [T, S, H, 512]; the pair and stream families write partials
-                          // instead of the output whenever it is given, with split 1 too
+  float* part_num;        // split > 1: [T, S, H, 512]
   float* part_max;        // split > 1: [T, S, H]
   float* part_sum;        // split > 1: [T, S, H]
   // Union launch of the pair family (heads = 128 rows of 128 / H queries):
@@ -76,8 +75,9 @@ struct FwdParams {
   unsigned long long wait_limit_ns;
   int wait_test;
   // The launch may run beside the kernel before it in the stream, on which
-  // nothing here depends, one item per cluster or CTA; it ends after that
-  // kernel, for which its last CTAs wait (pair and stream families).
+  // nothing here depends, one item per cluster or CTA; every split's partials
+  // are kept (split 1 too), and it ends after that kernel, for which its last
+  // CTAs wait (pair and stream families).
   int beside_previous;
 };
 
@@ -227,9 +227,7 @@ int umma_cluster_split(long long clusters, int split);
 cudaError_t launch_fwd_pair(const FwdParams& p, cudaStream_t stream);
 // CTAs of the pair family (two per cluster) resident at once (-1 on error).
 int pair_max_ctas();
-// `merge`: splits that fit a cluster merge their partials in the launch;
-// without it every split's partials are left for the caller.
-cudaError_t launch_fwd_stream(const FwdParams& p, cudaStream_t stream, bool merge = true);
+cudaError_t launch_fwd_stream(const FwdParams& p, cudaStream_t stream);
 cudaError_t launch_fwd_keys(const FwdParams& p, cudaStream_t stream);
 cudaError_t launch_fwd_pair_union(const FwdParams& p, cudaStream_t stream);
 cudaError_t launch_union_build(const int32_t* ids, int topk, int length, int qpb, int blocks, int32_t* uent,

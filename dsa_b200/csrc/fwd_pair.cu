@@ -361,7 +361,9 @@ __device__ __forceinline__ void issuer_q_chunks(int i, int* c0, int* c1) {
 
 // kUnion: the union launch (keys from per-block union entries, one
 // validity mask per query of the block); otherwise one index row per item.
-template <bool kUnion>
+// kBeside: the launch beside another kernel (FwdParams::beside_previous):
+// partials for every split, split 1 too, and an end after that kernel's.
+template <bool kUnion, bool kBeside = false>
 __global__ void __launch_bounds__(kPrThreads, 1) fwd_pair_kernel(const FwdParams p) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
@@ -755,7 +757,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) fwd_pair_kernel(const FwdParams
         if (e != 0) continue;
         const float f = (m_true == kNegFltMax) ? 1.f : ex2((m_w - m_true) * c);
         const size_t orow = (size_t)w.token * kPrHeads + row;
-        if (p.part_num == nullptr) {
+        if (!kBeside && p.split == 1) {
           p.out_max[orow] = final_max(m_true, l, p.scale_div);
           p.out_sum[orow] = l * f;
         } else {
@@ -921,7 +923,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) fwd_pair_kernel(const FwdParams
         if (!(ok = wait_warp(bar(kVFree0 + gl % kVStages), (gl / kVStages) & 1u, abort_flag))) break;
         tc_fence_after();
         const size_t orow = (size_t)w.token * kPrHeads + row;
-        if (p.part_num == nullptr) {
+        if (!kBeside && p.split == 1) {
           // O * (1/l) with the correctly rounded reciprocal (within an FP32 ulp of
           // O / l); a row without a valid index (l == 0) is written as 0
           const float rl = lf.x > 0.f ? __frcp_rn(lf.x) : 0.f;
@@ -942,13 +944,20 @@ __global__ void __launch_bounds__(kPrThreads, 1) fwd_pair_kernel(const FwdParams
         } else {
           const size_t pr = ((size_t)w.token * p.split + w.sp) * kPrHeads + row;
           float* dst = p.part_num + pr * kDimLatent;
-          const bool wide = (reinterpret_cast<uintptr_t>(p.part_num) & 31u) == 0;
 #pragma unroll 1
           for (int cb = cb0; cb < cb1; cb += 32) {
             uint32_t o[32];
             tmem_ld32(tmem + t_lane + kTmemO + cb, o);
             tmem_wait_ld();
-            store_f32_row32(dst + cb, o, lf.y, wide);
+            if constexpr (kBeside) {
+              store_f32_row32(dst + cb, o, lf.y, true);  // 32-byte aligned: the join's workspace is
+            } else {
+              float4* d4 = reinterpret_cast<float4*>(dst + cb);
+#pragma unroll
+              for (int k = 0; k < 8; ++k)
+                d4[k] = make_float4(u2f(o[4 * k]) * lf.y, u2f(o[4 * k + 1]) * lf.y, u2f(o[4 * k + 2]) * lf.y,
+                                    u2f(o[4 * k + 3]) * lf.y);
+            }
           }
         }
         tc_fence_before();
@@ -958,7 +967,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) fwd_pair_kernel(const FwdParams
     }
   }
   if (!ok && lane == 0) report_error(p.status, kErrTimeout);
-  if (p.beside_previous && cid == ncl - 1) grid_dependency_wait();
+  if constexpr (kBeside)
+    if (cid == ncl - 1) grid_dependency_wait();
 
   __syncwarp();
   tc_fence_before();
@@ -969,14 +979,11 @@ __global__ void __launch_bounds__(kPrThreads, 1) fwd_pair_kernel(const FwdParams
   }
 }
 
-// attr: two entries, the second used when cfg->numAttrs is raised to 2.
 bool pair_launch_config(cudaLaunchConfig_t* cfg, cudaLaunchAttribute* attr, int ctas, cudaStream_t stream) {
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 2;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  attr->id = cudaLaunchAttributeClusterDimension;
+  attr->val.clusterDim.x = 2;
+  attr->val.clusterDim.y = 1;
+  attr->val.clusterDim.z = 1;
   *cfg = cudaLaunchConfig_t{};
   cfg->gridDim = dim3((unsigned)ctas, 1, 1);
   cfg->blockDim = dim3(kPrThreads, 1, 1);
@@ -999,12 +1006,12 @@ int pair_max_ctas() {
           cudaSuccess)
     return -1;
   cudaLaunchConfig_t cfg;
-  cudaLaunchAttribute attr[2];
+  cudaLaunchAttribute attr;
   int dev = 0, sms = 0;
   if (cudaGetDevice(&dev) != cudaSuccess ||
       cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0)
     return -1;
-  pair_launch_config(&cfg, attr, sms & ~1, nullptr);
+  pair_launch_config(&cfg, &attr, sms & ~1, nullptr);
   int clusters = 0;
   if (cudaOccupancyMaxActiveClusters(&clusters, fwd_pair_kernel<false>, &cfg) != cudaSuccess || clusters <= 0)
     return -1;
@@ -1012,18 +1019,33 @@ int pair_max_ctas() {
   return cached;
 }
 
+// Beside the kernel before it in the stream: a cluster per item, which start
+// as SMs become free.
+static cudaError_t launch_fwd_pair_beside(const FwdParams& p, cudaStream_t stream) {
+  const long long items = (long long)p.tokens * p.split;
+  if (p.part_num == nullptr || items <= 0 || 2 * items > 0x7fffffffLL) return cudaErrorInvalidValue;
+  const cudaError_t err = cudaFuncSetAttribute(fwd_pair_kernel<false, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               (int)kSmemBytes);
+  if (err != cudaSuccess) return err;
+  cudaLaunchConfig_t cfg;
+  cudaLaunchAttribute attr[2];
+  pair_launch_config(&cfg, attr, (int)(2 * items), stream);
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, fwd_pair_kernel<false, true>, p);
+}
+
 cudaError_t launch_fwd_pair(const FwdParams& p, cudaStream_t stream) {
   if (p.heads != kPrHeads || p.keys_per_tile != kPrBN || p.uent != nullptr) return cudaErrorInvalidValue;
+  if (p.beside_previous) return launch_fwd_pair_beside(p, stream);
   const int max_ctas = pair_max_ctas();
   if (max_ctas <= 0) return cudaErrorInvalidConfiguration;
   const long long items = (long long)p.tokens * p.split;
-  // beside another kernel: a cluster per item, which start as SMs become free
-  const long long clusters = p.beside_previous || items < max_ctas / 2 ? items : max_ctas / 2;
-  if (2 * clusters > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
+  const long long clusters = items < max_ctas / 2 ? items : max_ctas / 2;
   cudaLaunchConfig_t cfg;
-  cudaLaunchAttribute attr[2];
-  pair_launch_config(&cfg, attr, (int)(2 * clusters), stream);
-  if (p.beside_previous) cfg.numAttrs = 2;
+  cudaLaunchAttribute attr;
+  pair_launch_config(&cfg, &attr, (int)(2 * clusters), stream);
   return cudaLaunchKernelEx(&cfg, fwd_pair_kernel<false>, p);
 }
 
@@ -1038,8 +1060,8 @@ cudaError_t launch_fwd_pair_union(const FwdParams& p, cudaStream_t stream) {
   const long long items = p.tokens;
   const long long clusters = items < max_ctas / 2 ? items : max_ctas / 2;
   cudaLaunchConfig_t cfg;
-  cudaLaunchAttribute attr[2];
-  pair_launch_config(&cfg, attr, (int)(2 * clusters), stream);
+  cudaLaunchAttribute attr;
+  pair_launch_config(&cfg, &attr, (int)(2 * clusters), stream);
   return cudaLaunchKernelEx(&cfg, fwd_pair_kernel<true>, p);
 }
 

@@ -219,7 +219,9 @@ __device__ __forceinline__ void stream_cluster_merge(const FwdParams& p, bool li
 // kCM: the cluster-merge launch (one item per CTA, the split CTAs of a
 // (token, head group) as one cluster, stream_cluster_merge at the end);
 // otherwise persistent CTAs and merge_kernel for split > 1.
-template <bool kCM>
+// kBeside: the launch beside another kernel (FwdParams::beside_previous), as
+// in the pair family.
+template <bool kCM, bool kBeside = false>
 __global__ void __launch_bounds__(kStThreads, 2) fwd_stream_kernel(const FwdParams p) {
   extern __shared__ __align__(128) unsigned char smem_raw[];
   StSmem& sm = *reinterpret_cast<StSmem*>(smem_raw);
@@ -485,7 +487,7 @@ __global__ void __launch_bounds__(kStThreads, 2) fwd_stream_kernel(const FwdPara
 
     // ---- epilogue (sm.m / sm.l final after the last softmax barrier) ----
     const float l0 = sm.l[g], l1 = sm.l[g + 8];
-    if (p.part_num == nullptr) {
+    if (!kBeside && p.split == 1) {
       // a row without a valid index (l == 0, O == 0) is written as 0 (O / inf)
       const float d0 = l0 > 0.f ? l0 : INFINITY, d1 = l1 > 0.f ? l1 : INFINITY;
       __nv_bfloat16* o0 = p.out + ((size_t)w.token * p.heads + h0 + g) * kDimLatent + cw * 128 + tq * 2;
@@ -517,7 +519,8 @@ __global__ void __launch_bounds__(kStThreads, 2) fwd_stream_kernel(const FwdPara
     }
   }
   if (failed && ctid == 0) report_error(p.status, kErrTimeout);
-  if (p.beside_previous && blockIdx.x == gridDim.x - 1) grid_dependency_wait();
+  if constexpr (kBeside)
+    if (blockIdx.x == gridDim.x - 1) grid_dependency_wait();
   if constexpr (kCM) stream_cluster_merge(p, !(*abort_flag) && !*reinterpret_cast<volatile int*>(&sm.stop));
 }
 
@@ -591,11 +594,29 @@ bool stream_cluster_merge(int split) {
   return cached[split] > 0;
 }
 
-cudaError_t launch_fwd_stream(const FwdParams& p, cudaStream_t stream, bool merge) {
+cudaError_t launch_fwd_stream(const FwdParams& p, cudaStream_t stream) {
   if (p.heads % kStHeads != 0 || p.keys_per_tile != kStBN) return cudaErrorInvalidValue;
   const long long items = (long long)p.tokens * (p.heads / kStHeads) * p.split;
   if (items <= 0 || items > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
-  if (merge && p.split > 1 && stream_cluster_merge(p.split)) {
+  if (p.beside_previous) {  // a CTA per item, which start as SMs become free
+    if (p.part_num == nullptr) return cudaErrorInvalidValue;
+    const int smem = (int)sizeof(StSmem);
+    const cudaError_t err =
+        cudaFuncSetAttribute(fwd_stream_kernel<false, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (err != cudaSuccess) return err;
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3((unsigned)items, 1, 1);
+    cfg.blockDim = dim3(kStThreads, 1, 1);
+    cfg.dynamicSmemBytes = sizeof(StSmem);
+    cfg.stream = stream;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, fwd_stream_kernel<false, true>, p);
+  }
+  if (p.split > 1 && stream_cluster_merge(p.split)) {
     cudaLaunchConfig_t cfg;
     cudaLaunchAttribute attr;
     st_cm_launch_config(&cfg, &attr, p.split, items, stream);
@@ -603,21 +624,7 @@ cudaError_t launch_fwd_stream(const FwdParams& p, cudaStream_t stream, bool merg
   }
   const int max_ctas = stream_max_ctas();
   if (max_ctas <= 0) return cudaErrorInvalidConfiguration;
-  // beside another kernel: a CTA per item, which start as SMs become free
-  const int ctas = (int)(p.beside_previous || items < max_ctas ? items : max_ctas);
-  if (p.beside_previous) {
-    cudaLaunchConfig_t cfg{};
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = dim3((unsigned)ctas, 1, 1);
-    cfg.blockDim = dim3(kStThreads, 1, 1);
-    cfg.dynamicSmemBytes = sizeof(StSmem);
-    cfg.stream = stream;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, fwd_stream_kernel<false>, p);
-  }
+  const int ctas = (int)(items < max_ctas ? items : max_ctas);
   fwd_stream_kernel<false><<<ctas, kStThreads, sizeof(StSmem), stream>>>(p);
   return cudaGetLastError();
 }
