@@ -249,44 +249,42 @@ struct Maps {
   CUtensorMap rope;  // rope, boxes of 64 / G keys x 64 dims
 };
 
-// Chunks [c0, c0 + N) (dims 64c..; chunk 8: rope) of the 32 Q rows of this
-// warp -> TMEM, lane = row, 32 columns a chunk. The loads take whole 128-byte
-// lines, four rows an instruction (a lane reading its own row costs 32 line
-// lookups an instruction: 8,900 cycles for Q against 2,500), all chunks in flight
-// together; each goes through 4 KB of shared memory (swizzled) to become rows.
-template <int N>
-__device__ __forceinline__ void load_q_chunks(const PrefixParams& p, long long row0, int lane, int c0, uint4 (*v)[8]) {
-#pragma unroll
-  for (int i = 0; i < N; ++i)
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const size_t row = (size_t)min(row0 + 4 * k + (lane >> 3), p.rows - 1);  // rows past the end repeat the last one
-      v[i][k] = __ldg((c0 + i < 8 ? reinterpret_cast<const uint4*>(p.q + row * kDimLatent) + (c0 + i) * 8
-                                  : reinterpret_cast<const uint4*>(p.q_rope + row * kDimRope)) + (lane & 7));
-    }
-}
-template <int N>
-__device__ __forceinline__ void store_q_chunks(int lane, int c0, const uint4 (*v)[8], uint8_t* scratch, uint32_t tq) {
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int r = 4 * k + (lane >> 3);
-      *reinterpret_cast<uint4*>(scratch + r * 128 + (((lane & 7) ^ (r & 7)) * 16)) = v[i][k];
-    }
-    __syncwarp();
-    uint32_t out[32];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const uint4 w = *reinterpret_cast<const uint4*>(scratch + lane * 128 + ((k ^ (lane & 7)) * 16));
-      out[4 * k] = w.x;
-      out[4 * k + 1] = w.y;
-      out[4 * k + 2] = w.z;
-      out[4 * k + 3] = w.w;
-    }
-    tmem_st32(tq + (uint32_t)(c0 + i) * 32u, out);
-    __syncwarp();
+// Q of a warp's 32 rows -> TMEM, lane = row, 32 columns per chunk of 64 dims
+// (chunk 8: rope). The loads take whole 128-byte lines, four rows an
+// instruction (a lane reading its own row costs 32 line lookups an instruction:
+// 8,900 cycles for Q), and all of a warp's chunks are in flight together, two
+// into shared memory and the rest into registers; a chunk goes through 4 KB of
+// shared memory (swizzled) to become rows.
+struct QRows {
+  const uint8_t *latent, *rope;  // this lane's 16 bytes of the warp's first row
+  int first, last;               // this lane's row of piece 0, the last row that is there (later ones repeat it)
+  __device__ __forceinline__ QRows(const PrefixParams& p, long long row0, int lane) {
+    const long long at = min(row0, p.rows - 1);
+    latent = reinterpret_cast<const uint8_t*>(p.q + at * kDimLatent) + (lane & 7) * 16;
+    rope = reinterpret_cast<const uint8_t*>(p.q_rope + at * kDimRope) + (lane & 7) * 16;
+    first = lane >> 3;
+    last = (int)min(p.rows - 1 - at, 31LL);
   }
+  __device__ __forceinline__ const uint4* piece(int c, int k) const {  // rows 4 k ..  of chunk c
+    const int r = min(first + 4 * k, last);
+    return reinterpret_cast<const uint4*>(c < 8 ? latent + r * 1024 + c * 128 : rope + r * 128);
+  }
+};
+__device__ __forceinline__ uint32_t q_place(int lane, int k) {  // of piece k of a chunk in its 4 KB
+  const int r = 4 * k + (lane >> 3);
+  return (uint32_t)(r * 128 + (((lane & 7) ^ (r & 7)) * 16));
+}
+__device__ __forceinline__ void q_to_tmem(int lane, const uint8_t* scratch, uint32_t taddr) {
+  uint32_t out[32];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const uint4 w = *reinterpret_cast<const uint4*>(scratch + lane * 128 + ((k ^ (lane & 7)) * 16));
+    out[4 * k] = w.x;
+    out[4 * k + 1] = w.y;
+    out[4 * k + 2] = w.z;
+    out[4 * k + 3] = w.w;
+  }
+  tmem_st32(taddr, out);
 }
 
 // Split cluster barrier: what this thread wrote before the arrive is visible
@@ -346,10 +344,26 @@ __global__ void __launch_bounds__(kPxThreads, 1) fwd_prefix_kernel(const PrefixP
     return;
   }
 
-  // the softmax warps' first two chunks of Q are under way while the CTA sets up
-  uint4 q_first[3][8];
-  if (score && warp >= kSoftWarp0)
-    load_q_chunks<2>(p, row0 + (warp & 3) * 32, lane, 5 * ((warp - kSoftWarp0) >> 2), q_first);
+  // the softmax warps' chunks of Q are under way while the CTA sets up: group 0
+  // takes chunks 0-4, group 1 5-8, the first two through shared memory (in the P
+  // staging slots: P of a tile is written after every warp's Q is in TMEM)
+  const int q_group = (warp - kSoftWarp0) >> 2;
+  const uint32_t q_scratch = C::kOffLocal + (uint32_t)(warp - kSoftWarp0) * 8192u;
+  uint4 q_rest[3][8];
+  if (score && warp >= kSoftWarp0) {
+    const QRows rows(p, row0 + (warp & 3) * 32, lane);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        cp_async_16(base + q_scratch + (uint32_t)i * 4096u + q_place(lane, k), rows.piece(5 * q_group + i, k));
+    cp_async_commit();
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+      if (i < 2 || q_group == 0)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) q_rest[i][k] = __ldg(rows.piece(5 * q_group + 2 + i, k));
+  }
   // one barrier per thread (each CTA uses its own part of them)
   if (threadIdx.x < C::kBarCount) mbar_init(bar((int)threadIdx.x), C::bar_count((int)threadIdx.x));
   if (threadIdx.x == 0) *abort_flag = 0;
@@ -470,16 +484,21 @@ __global__ void __launch_bounds__(kPxThreads, 1) fwd_prefix_kernel(const PrefixP
       float* const mpub = reinterpret_cast<float*>(sbase + C::kOffM);
       float* const xch = reinterpret_cast<float*>(sbase + C::kOffX);
       {
-        // scratch in the P staging slots: P of a tile is written after every warp's Q is loaded
-        uint8_t* const scratch = sbase + C::kOffLocal + (warp - kSoftWarp0) * 4096;
-        const uint32_t tq = tmem + t_lane + kTmemQ;
-        store_q_chunks<2>(lane, 5 * e, q_first, scratch, tq);
-        if (e == 0) {
-          load_q_chunks<3>(p, row0 + quad * 32, lane, 2, q_first);
-          store_q_chunks<3>(lane, 2, q_first, scratch, tq);
-        } else {
-          load_q_chunks<2>(p, row0 + quad * 32, lane, 7, q_first);
-          store_q_chunks<2>(lane, 7, q_first, scratch, tq);
+        uint8_t* const scratch = sbase + q_scratch;
+        const uint32_t tq = tmem + t_lane + kTmemQ + (uint32_t)e * 160u;  // chunk 5 e
+        cp_async_wait<0>();
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 2; ++i) q_to_tmem(lane, scratch + i * 4096, tq + (uint32_t)i * 32u);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+          if (i == 2 && e != 0) break;
+          uint8_t* const at = scratch + (i & 1) * 4096;
+          __syncwarp();  // what was there has been read
+#pragma unroll
+          for (int k = 0; k < 8; ++k) *reinterpret_cast<uint4*>(at + q_place(lane, k)) = q_rest[i][k];
+          __syncwarp();
+          q_to_tmem(lane, at, tq + (uint32_t)(2 + i) * 32u);
         }
         tmem_wait_st();
         tc_fence_before();

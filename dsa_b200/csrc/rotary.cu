@@ -117,6 +117,30 @@ struct Two<T, 1> {
   }
 };
 
+// Elements at which the two vectors of unit u start: a rotary unit's, or (from
+// units_rot on) two of the copied vectors, of which the second may be missing.
+template <int V, bool kHalf>
+__device__ __forceinline__ void place(const RotaryParams& p, int u, int units_rot, int units, int* o0, int* o1, bool* two) {
+  *two = true;
+  if (u < units_rot) {
+    *o0 = p.start + (V == 1 && !kHalf ? 2 * u : u * V);
+    *o1 = V == 1 && !kHalf ? *o0 + 1 : *o0 + p.rotary_dim / 2;
+  } else {
+    const int vecs = (p.dim - p.rotary_dim) / V, first = p.start / V, skip = p.rotary_dim / V;
+    const int c0 = u - units_rot, c1 = c0 + units - units_rot;
+    *two = c1 < vecs;
+    *o0 = (c0 + (c0 >= first ? skip : 0)) * V;
+    *o1 = (c1 + (c1 >= first ? skip : 0)) * V;
+  }
+}
+// The q-th of the V pairs of rotary unit u: with V > 1 and interleaved pairs,
+// V / 2 in each of its two vectors, else one element in each.
+template <int V, bool kHalf>
+__device__ __forceinline__ int pair_of(const RotaryParams& p, int u, int q) {
+  if (V == 1 || kHalf) return u * V + q;
+  return q < V / 2 ? u * (V / 2) + q : p.rotary_dim / 4 + u * (V / 2) + q - V / 2;
+}
+
 // V: elements of a vector (16 bytes' worth, or 1 for sizes, strides or
 // addresses that 16-byte accesses do not fit).
 template <typename T, int V, bool kHalf>
@@ -134,20 +158,10 @@ __global__ void __launch_bounds__(kRoThreads) rotary_kernel(const RotaryParams p
   const T* x = static_cast<const T*>(p.x) + b * p.xs[0] + s * p.xs[1] + g * p.xs[2];
   T* y = static_cast<T*>(p.y) + b * p.ys[0] + s * p.ys[1] + g * p.ys[2];
 
-  // this thread's two vectors: of a rotary unit, or copied ones
   const bool turns = u < units_rot;
   int o0, o1;
-  bool two = true;
-  if (turns) {
-    o0 = p.start + (V == 1 && !kHalf ? 2 * u : u * V);
-    o1 = V == 1 && !kHalf ? o0 + 1 : o0 + p.rotary_dim / 2;
-  } else {
-    const int vecs = (p.dim - p.rotary_dim) / V, first = p.start / V, skip = p.rotary_dim / V;
-    const int c0 = u - units_rot, c1 = c0 + units - units_rot;
-    two = c1 < vecs;
-    o0 = (c0 + (c0 >= first ? skip : 0)) * V;
-    o1 = (c1 + (c1 >= first ? skip : 0)) * V;
-  }
+  bool two;
+  place<V, kHalf>(p, u, units_rot, units, &o0, &o1, &two);
   Two<T, V> cur;
   if (live) cur.load(x, o0, o1, two);
 
@@ -174,9 +188,7 @@ __global__ void __launch_bounds__(kRoThreads) rotary_kernel(const RotaryParams p
   float2 cs[V];
   if (turns) {
 #pragma unroll
-    for (int q = 0; q < V; ++q)
-      cs[q] = table[k * pairs + (V == 1 || kHalf ? u * V + q
-                                                 : q < V / 2 ? u * (V / 2) + q : p.rotary_dim / 4 + u * (V / 2) + q - V / 2)];
+    for (int q = 0; q < V; ++q) cs[q] = table[k * pairs + pair_of<V, kHalf>(p, u, q)];
   }
   for (int h = g;;) {  // the next head's loads are under way while this one is turned
     Two<T, V> next;
@@ -190,11 +202,68 @@ __global__ void __launch_bounds__(kRoThreads) rotary_kernel(const RotaryParams p
   }
 }
 
+// One head a token (k_rope, the indexer's keys): nobody shares a token's
+// cosines, so a thread computes those of its pairs itself; the block keeps the
+// pairs' turn fractions. Rotary units and copied ones are in different warps
+// where they are many (cosines for half a warp cost as much as for a whole one).
+template <typename T, int V, bool kHalf>
+__global__ void __launch_bounds__(kRoThreads, 4) rotary_rows_kernel(const RotaryParams p, int units_rot, int units,
+                                                                    int tokens_per_block) {
+  extern __shared__ unsigned long long fractions[];  // [rotary_dim / 2]
+  const int tid = (int)threadIdx.x, rotary = tokens_per_block * units_rot;
+  const bool turns = tid < rotary;
+  const int mine = turns ? tid : tid - rotary, per_token = turns ? units_rot : units - units_rot;
+  const int k = per_token > 0 ? mine / per_token : tokens_per_block;
+  const int u = mine - k * per_token + (turns ? 0 : units_rot);
+  const bool live = k < tokens_per_block;
+  int o0 = 0, o1 = 0;
+  bool two = false;
+  if (live) place<V, kHalf>(p, u, units_rot, units, &o0, &o1, &two);
+  const uint32_t stride = gridDim.x * (uint32_t)tokens_per_block, tokens = (uint32_t)p.tokens;  // < 2^31, stride < 2^20
+  Two<T, V> cur;
+  long long pos = 0;
+  uint32_t b = 0, s = 0;
+  auto load = [&](uint32_t t) {
+    b = t / (uint32_t)p.queries;
+    s = t - b * (uint32_t)p.queries;
+    cur.load(static_cast<const T*>(p.x) + b * p.xs[0] + s * p.xs[1], o0, o1, two);
+    if (turns) {
+      const long long i = b * p.ps[0] + s * p.ps[1];
+      pos = p.pos64 ? static_cast<const long long*>(p.positions)[i] : (long long)static_cast<const int32_t*>(p.positions)[i];
+    }
+  };
+  uint32_t t = live ? blockIdx.x * (uint32_t)tokens_per_block + (uint32_t)k : tokens;
+  if (t < tokens) load(t);
+  for (int j = tid; j < p.rotary_dim / 2; j += kRoThreads) fractions[j] = turn_fraction(__ldg(p.inv_freq + j));
+  __syncthreads();
+  while (t < tokens) {
+    if (turns) {
+      float2 cs[V];
+#pragma unroll
+      for (int q = 0; q < V; ++q)
+        rotary_cos_sin(pos, fractions[pair_of<V, kHalf>(p, u, q)], p.factor, p.sin_sign, &cs[q].x, &cs[q].y);
+      cur.template turn<kHalf>(cs);
+    }
+    cur.store(static_cast<T*>(p.y) + b * p.ys[0] + s * p.ys[1], o0, o1, two);
+    t += stride;
+    if (t < tokens) load(t);
+  }
+}
+
 template <typename T, int V>
 cudaError_t launch_v(const RotaryParams& p, cudaStream_t stream) {
   const int units_rot = p.rotary_dim / (2 * V);
   const int copies = p.in_place ? 0 : (p.dim - p.rotary_dim) / V;
   const int units = units_rot + (copies + 1) / 2;
+  if (p.heads == 1 && units <= kRoThreads) {
+    const int per_block = kRoThreads / units;
+    long long blocks = (p.tokens + per_block - 1) / per_block;
+    if (blocks > 148 * 16) blocks = 148 * 16;
+    const size_t smem = (size_t)(p.rotary_dim / 2) * sizeof(unsigned long long);
+    if (p.half) rotary_rows_kernel<T, V, true><<<(unsigned)blocks, kRoThreads, smem, stream>>>(p, units_rot, units, per_block);
+    else rotary_rows_kernel<T, V, false><<<(unsigned)blocks, kRoThreads, smem, stream>>>(p, units_rot, units, per_block);
+    return cudaGetLastError();
+  }
   // heads per thread: one while that leaves a part of the GPU idle, then as
   // many as keep it full (148 SMs x 2048 threads), so that a block's cosines
   // serve more rows. 4096 tokens x 64 heads x 128 (64 turned): 23.4 us, with

@@ -1,9 +1,10 @@
 """GPU parity of the rotary operator against its definition in FP64.
 
-Tolerances: a cosine or sine is the FP32 sincospif of an angle rounded to
-2^-24 of a half turn, so off by at most pi * 2^-24 + 2^-22 (two FP32 steps of a
-value near 1, as CUDA's documented 2 ulp) < 2^-21 with the factor's rounding
-counted once more at 2^-24; a result adds two products of FP32 rounding:
+Tolerances: a cosine or sine is off by at most 1.0e-7 (polynomials of an angle
+reduced exactly and rounded to 2^-24 of an eighth of a turn, see the kernel)
+and by the factor's rounding, 2^-24, together below 2^-22; 2^-21 leaves room
+for the FP64 reference's own angle at positions near 2^31 (2^31 * 2^-53 < 2^-21.9).
+A result adds two products of FP32 rounding:
 |error| <= f (|a| + |b|) (2^-21 + 3 * 2^-24) plus half a step of the type.
 """
 import pytest
@@ -48,7 +49,7 @@ def _make(shape, dtype, seed, far=100000):
 @pytest.mark.parametrize("shape,rotary_dim,start", [
     ((1, 1, 1, 64), 64, 0), ((3, 5, 7, 64), 64, 0), ((1, 9, 64, 128), 64, 0), ((2, 3, 16, 192), 64, 128),
     ((2, 129, 2, 96), 32, 32), ((2, 3, 5, 11), 6, 3), ((1, 1, 1, 2), 2, 0), ((2, 2, 3, 30), 30, 0), ((2, 7, 576), 64, 512),
-    ((1, 2, 300, 64), 64, 0), ((70, 130, 3, 72), 64, 8), ((1, 1, 1, 1024), 1024, 0), ((2, 3, 2, 4096), 4096, 0), ((1, 2, 3, 65536), 64, 65000), ((1, 1, 40000, 66), 66, 0), ((4, 40, 128, 24), 16, 8)])
+    ((1, 2, 300, 64), 64, 0), ((3, 7000, 1, 64), 64, 0), ((2, 3000, 128), 64, 0), ((5, 999, 1, 17), 10, 3), ((2, 5, 1, 4096), 64, 64), ((70, 130, 3, 72), 64, 8), ((1, 1, 1, 1024), 1024, 0), ((2, 3, 2, 4096), 4096, 0), ((1, 2, 3, 65536), 64, 65000), ((1, 1, 40000, 66), 66, 0), ((4, 40, 128, 24), 16, 8)])
 def test_rotary(cuda_lib, shape, rotary_dim, start, dtype, layout):
     x, pos = _make(shape, dtype, sum(shape))
     freq = dsa_b200.rotary_frequencies(rotary_dim, device="cuda")
