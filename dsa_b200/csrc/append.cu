@@ -85,8 +85,8 @@ __device__ __forceinline__ void write_row(const AppendParams& p, long long slot,
     const float scale = amax > 0.f ? __fdiv_rn(amax, 448.f) : 1.f;
     // kv / scale, correctly rounded: with the correctly rounded reciprocal one
     // Newton step on the quotient's exact remainder gives it (Markstein, 1990)
-    // while nothing leaves the normal range (a zero keeps its sign by hand);
-    // 16 divisions would cost a lane more than all the rest.
+    // while nothing leaves the normal range; 16 divisions would cost a lane
+    // more than all the rest.
     uint32_t q[4];
     if (top < 0x7f80u && scale >= 0x1p-60f && scale <= 0x1p60f) {  // every value finite
       const float inv = __frcp_rn(scale);
@@ -97,7 +97,7 @@ __device__ __forceinline__ void write_row(const AppendParams& p, long long slot,
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float y = __fmul_rn(x[i], inv);
-          x[i] = copysignf(__fmaf_rn(__fmaf_rn(-y, scale, x[i]), inv, y), y);
+          x[i] = __fmaf_rn(-__fmaf_rn(y, scale, -x[i]), inv, y);  // in these signs a zero keeps its own
         }
         q[k] = pack_e4m3(x);
       }
@@ -131,30 +131,22 @@ __device__ __forceinline__ void write_row(const AppendParams& p, long long slot,
   }
 }
 
-// A warp walks over tokens; the next token's row and the slot of the one after
-// it are under way while a row is written.
+// A warp walks over tokens. Eight blocks an SM hide the loads; keeping the next
+// token's row under way in registers instead (five blocks) measured 19.1 us
+// against 18.0 for 65536 FP8 tokens.
 template <bool kFp8, bool kWide>
-__global__ void __launch_bounds__(kApThreads, 5) append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(kApThreads, 8) append_kernel(const AppendParams p) {
   const int lane = threadIdx.x & 31;
   const uint32_t stride = gridDim.x * (kApThreads / 32);
   const uint32_t tokens = (uint32_t)p.tokens;  // < 2^31
   const int e0 = p.half ? lane : 2 * lane, e1 = p.half ? lane + 32 : 2 * lane + 1;
   const unsigned long long fraction = p.inv_freq != nullptr ? turn_fraction(__ldg(p.inv_freq + lane)) : 0;
-  auto slot_of = [&](uint32_t t) -> long long {
-    const int32_t slot = t < tokens ? __ldg(p.slots + t) : -1;
-    return slot < p.rows ? slot : -1;
-  };
-  uint32_t t = blockIdx.x * (kApThreads / 32) + (threadIdx.x >> 5);
-  long long slot = slot_of(t), slot_nx = slot_of(t + stride);
-  Row cur, nx;
-  if (slot >= 0) load_row<kWide>(p, t, lane, e0, e1, cur);
-  for (; t < tokens; t += stride) {
-    const long long slot_nx2 = slot_of(t + 2 * stride);
-    if (slot_nx >= 0) load_row<kWide>(p, t + stride, lane, e0, e1, nx);
-    if (slot >= 0) write_row<kFp8>(p, slot, lane, e0, e1, fraction, cur);
-    slot = slot_nx;
-    slot_nx = slot_nx2;
-    cur = nx;
+  for (uint32_t t = blockIdx.x * (kApThreads / 32) + (threadIdx.x >> 5); t < tokens; t += stride) {
+    const int32_t slot = __ldg(p.slots + t);
+    if (slot < 0 || slot >= p.rows) continue;
+    Row row;
+    load_row<kWide>(p, t, lane, e0, e1, row);
+    write_row<kFp8>(p, slot, lane, e0, e1, fraction, row);
   }
 }
 
@@ -162,7 +154,7 @@ __global__ void __launch_bounds__(kApThreads, 5) append_kernel(const AppendParam
 
 cudaError_t launch_append_kv(const AppendParams& p, cudaStream_t stream) {
   long long blocks = (p.tokens + kApThreads / 32 - 1) / (kApThreads / 32);
-  if (blocks > 148 * 5) blocks = 148 * 5;
+  if (blocks > 148 * 16) blocks = 148 * 16;
   bool wide = (reinterpret_cast<uintptr_t>(p.kv) & 15u) == 0 && p.kvs[0] % 8 == 0 && p.kvs[1] % 8 == 0;
   const unsigned g = (unsigned)blocks;
   if (p.cache != nullptr) {
