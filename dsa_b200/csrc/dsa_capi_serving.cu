@@ -77,7 +77,7 @@ bool plan_prefix(const dsa_fwd_args_t* a, const dsa_prefix_kv_t* px, PrefixPlan*
   plan->row_tiles = (plan->rows + 127) / 128;
   int split1 = 1, split2 = 1;
   const double one = prefix_split(plan->row_tiles, px->rows, 1, &split1), two = prefix_split(plan->row_tiles, px->rows, 2, &split2);
-  plan->group = plan->row_tiles > 1 && two < one ? 2 : 1;
+  plan->group = two < one ? 2 : 1;
   plan->split = plan->group == 2 ? split2 : split1;
   if ((plan->row_tiles + 1) * plan->split > kMaxInt / 2) return false;
   plan->own_split = 0;
