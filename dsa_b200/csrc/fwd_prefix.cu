@@ -21,9 +21,9 @@
 // bounds G = 1: a tile writes and reads 72 KB of K and passes 17 KB of P in the
 // score CTA, writes and reads 64 KB of V and reads P twice in the value CTA,
 // 178 KB each at 128 bytes a cycle = 1,390 cycles (1,400 measured) against
-// 1,152 of MMA. G = 2 takes 1,190: 4096 rows over 32003 keys run at 1,445
-// TFLOP/s (0.87 of the measured cuBLAS burst, 1.05 of its sustained rate; G = 1
-// 1,290), 1024 rows over 32768, in nine splits, at 1,110 (G = 1 1,060).
+// 1,152 of MMA. G = 2 takes 1,190: 4096 rows over 32003 keys run at 1,480
+// TFLOP/s (0.89 of the measured cuBLAS burst, 1.08 of its sustained rate; G = 1
+// 1,170), 1024 rows over 32768, in eight splits, at 1,207 (G = 1 1,030).
 //
 // Keys come by TMA (one 3-D map that turns a row of 512 into eight 64-wide
 // blocks, 128-byte swizzle) in boxes of 32 KB / G, each released by the MMAs

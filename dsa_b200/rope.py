@@ -74,7 +74,7 @@ def _check_rope(positions, inv_freq, layout, attention_factor, lead, index):
     number = _native.ROPE_LAYOUTS.get(layout)
     if number is None:
         raise ValueError("layout must be 'interleaved' or 'half'")
-    if type(attention_factor) not in (float, int) or not math.isfinite(attention_factor):
+    if not isinstance(attention_factor, (float, int)) or isinstance(attention_factor, bool) or not math.isfinite(attention_factor):
         raise ValueError("attention_factor must be a finite number")
     if positions.shape != lead or positions.dtype not in _POSITIONS:
         raise ValueError("positions must be int32 or int64 and have one entry per token")
@@ -146,7 +146,8 @@ def rotary(x, positions, inv_freq, *, layout="interleaved", start=0, attention_f
     Returns a new contiguous tensor, or ``out`` (same shape and type; ``x``
     itself for an update in place). Without ``out`` the call is differentiable
     in ``x``; the gradient is one launch of the same kernel. Angles are reduced
-    in FP64, cosines and products are FP32, rounded once to the type of ``x``.
+    exactly (64-bit fractions of a turn), cosines and products are FP32, rounded
+    once to the type of ``x``; frequencies and the factor are finite.
     """
     shape = x.shape
     if len(shape) not in (3, 4) or 0 in shape:

@@ -236,7 +236,7 @@ DSA_B200_API int dsa_indexer_topk(const dsa_indexer_args_t* args, void* stream);
  * over the pairs (2i, 2i + 1) (interleaved) or (i, i + rotary_dim / 2) (half),
  * f = attention_factor, and -t when `inverse` is set (which is also the
  * gradient of the forward map). The other elements are copied. The angle is
- * reduced in FP64, cosines and products are FP32, one rounding to the type. y
+ * reduced exactly, cosines and products are FP32, one rounding to the type. y
  * may be x (same pointer and strides) and overlaps it in no other way. */
 typedef enum dsa_dtype { DSA_BF16 = 0, DSA_FP16 = 1, DSA_FP32 = 2 } dsa_dtype_t;
 typedef enum dsa_rope_layout { DSA_ROPE_INTERLEAVED = 0, DSA_ROPE_HALF = 1 } dsa_rope_layout_t;
