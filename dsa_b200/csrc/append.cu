@@ -37,9 +37,27 @@ __device__ __forceinline__ void load16(const __nv_bfloat16* src, uint4& a, uint4
   }
 }
 
-__device__ __forceinline__ uint32_t pack_e4m3(const float* x) {
-  return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(x[0], x[1]), __NV_SATFINITE, __NV_E4M3) |
-         ((uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(x[2], x[3]), __NV_SATFINITE, __NV_E4M3) << 16);
+__device__ __forceinline__ uint32_t pack_e4m3(float2 a, float2 b) {
+  return (uint32_t)__nv_cvt_float2_to_fp8x2(a, __NV_SATFINITE, __NV_E4M3) |
+         ((uint32_t)__nv_cvt_float2_to_fp8x2(b, __NV_SATFINITE, __NV_E4M3) << 16);
+}
+
+__device__ __forceinline__ unsigned long long pack_f32x2(float a, float b) {
+  unsigned long long v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+  return v;
+}
+
+// Minus the quotients of a word's two BF16 values by the scale; n is minus its reciprocal.
+__device__ __forceinline__ float2 quotient2(uint32_t w, unsigned long long scale, unsigned long long n) {
+  const unsigned long long x = pack_f32x2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  unsigned long long y, r;
+  float2 z;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(x), "l"(n));
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(y), "l"(scale), "l"(x));
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y) : "l"(r), "l"(n), "l"(y));
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(z.x), "=f"(z.y) : "l"(y));
+  return z;
 }
 
 // One token's row as a lane holds it.
@@ -52,7 +70,7 @@ struct Row {
 // kWide: kv rows start on 16-byte boundaries.
 template <bool kWide>
 __device__ __forceinline__ void load_row(const AppendParams& p, uint32_t t, int lane, int e0, int e1, Row& r) {
-  const uint32_t b = t / (uint32_t)p.queries, s = t - b * (uint32_t)p.queries;
+  const uint32_t b = p.queries != 0 ? t / (uint32_t)p.queries : 0, s = t - b * (uint32_t)p.queries;
   const __nv_bfloat16* const kr = p.k_rope + b * p.krs[0] + s * p.krs[1];
   load16<kWide>(p.kv + b * p.kvs[0] + s * p.kvs[1] + lane * 16, r.v0, r.v1);
   r.r0 = kr[e0];
@@ -82,33 +100,32 @@ __device__ __forceinline__ void write_row(const AppendParams& p, long long slot,
 #pragma unroll
     for (int d = 1; d < 8; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
     const float amax = __uint_as_float(top << 16);
-    const float scale = amax > 0.f ? __fdiv_rn(amax, 448.f) : 1.f;
+    float scale;
     // kv / scale, correctly rounded: with the correctly rounded reciprocal one
     // Newton step on the quotient's exact remainder gives it (Markstein, 1990)
     // while nothing leaves the normal range; 16 divisions would cost a lane
-    // more than all the rest.
+    // more than all the rest. Two values go through an instruction, negated:
+    // so an exact quotient's zero remainder leaves a zero its sign.
     uint32_t q[4];
-    if (top < 0x7f80u && scale >= 0x1p-60f && scale <= 0x1p60f) {  // every value finite
+    if (top < 0x7f80u && amax >= 0x1p-60f && amax <= 0x1p60f) {  // every value finite
+      constexpr float kInv = 1.f / 448.f;
+      scale = __fmul_rn(amax, kInv);
+      scale = __fmaf_rn(__fmaf_rn(scale, -448.f, amax), kInv, scale);
       const float inv = __frcp_rn(scale);
+      const unsigned long long s2 = pack_f32x2(scale, scale), n2 = pack_f32x2(-inv, -inv);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        float x[4] = {__uint_as_float(w[2 * k] << 16), __uint_as_float(w[2 * k] & 0xffff0000u),
-                      __uint_as_float(w[2 * k + 1] << 16), __uint_as_float(w[2 * k + 1] & 0xffff0000u)};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float y = __fmul_rn(x[i], inv);
-          x[i] = __fmaf_rn(-__fmaf_rn(y, scale, -x[i]), inv, y);  // in these signs a zero keeps its own
-        }
-        q[k] = pack_e4m3(x);
+        q[k] = pack_e4m3(quotient2(w[2 * k], s2, n2), quotient2(w[2 * k + 1], s2, n2)) ^ 0x80808080u;
       }
     } else {
+      scale = amax > 0.f ? __fdiv_rn(amax, 448.f) : 1.f;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const float x[4] = {__fdiv_rn(__uint_as_float(w[2 * k] << 16), scale),
                             __fdiv_rn(__uint_as_float(w[2 * k] & 0xffff0000u), scale),
                             __fdiv_rn(__uint_as_float(w[2 * k + 1] << 16), scale),
                             __fdiv_rn(__uint_as_float(w[2 * k + 1] & 0xffff0000u), scale)};
-        q[k] = pack_e4m3(x);
+        q[k] = pack_e4m3(make_float2(x[0], x[1]), make_float2(x[2], x[3]));
       }
     }
     reinterpret_cast<uint4*>(row)[lane] = make_uint4(q[0], q[1], q[2], q[3]);
@@ -131,18 +148,26 @@ __device__ __forceinline__ void write_row(const AppendParams& p, long long slot,
   }
 }
 
-// A warp walks over tokens. Eight blocks an SM hide the loads; keeping the next
-// token's row under way in registers instead (five blocks) measured 19.1 us
-// against 18.0 for 65536 FP8 tokens.
+// A warp walks over tokens, the next token's slot under way. Measured with FP8
+// rows: 151552 tokens 47.4 us (5.8 TB/s, near the copy rate), 32768 tokens
+// 12.3, 65536 of which half are padding 14.9 (warps meet unequal numbers of
+// those). Six blocks an SM, all of them resident, hide the loads; eight took
+// 50.3, 12.9 and 14.8, and two rounds of eight 15.3 for the last. Keeping the
+// next token's row in registers too (five blocks) was slower.
+constexpr int kApBlocks = 6;
+
 template <bool kFp8, bool kWide>
-__global__ void __launch_bounds__(kApThreads, 8) append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(kApThreads, kApBlocks) append_kernel(const AppendParams p) {
   const int lane = threadIdx.x & 31;
   const uint32_t stride = gridDim.x * (kApThreads / 32);
   const uint32_t tokens = (uint32_t)p.tokens;  // < 2^31
   const int e0 = p.half ? lane : 2 * lane, e1 = p.half ? lane + 32 : 2 * lane + 1;
   const unsigned long long fraction = p.inv_freq != nullptr ? turn_fraction(__ldg(p.inv_freq + lane)) : 0;
-  for (uint32_t t = blockIdx.x * (kApThreads / 32) + (threadIdx.x >> 5); t < tokens; t += stride) {
-    const int32_t slot = __ldg(p.slots + t);
+  uint32_t t = blockIdx.x * (kApThreads / 32) + (threadIdx.x >> 5);
+  int32_t next = t < tokens ? __ldg(p.slots + t) : -1;
+  for (; t < tokens; t += stride) {
+    const int32_t slot = next;
+    next = t + stride < tokens ? __ldg(p.slots + t + stride) : -1;
     if (slot < 0 || slot >= p.rows) continue;
     Row row;
     load_row<kWide>(p, t, lane, e0, e1, row);
@@ -154,7 +179,7 @@ __global__ void __launch_bounds__(kApThreads, 8) append_kernel(const AppendParam
 
 cudaError_t launch_append_kv(const AppendParams& p, cudaStream_t stream) {
   long long blocks = (p.tokens + kApThreads / 32 - 1) / (kApThreads / 32);
-  if (blocks > 148 * 16) blocks = 148 * 16;
+  if (blocks > 148 * kApBlocks) blocks = 148 * kApBlocks;
   bool wide = (reinterpret_cast<uintptr_t>(p.kv) & 15u) == 0 && p.kvs[0] % 8 == 0 && p.kvs[1] % 8 == 0;
   const unsigned g = (unsigned)blocks;
   if (p.cache != nullptr) {

@@ -219,7 +219,15 @@ int dsa_append_kv(const dsa_append_kv_args_t* a, void* stream) {
   }
   p.tokens = a->batch * a->queries;
   p.rows = a->rows;
+  // tokens that one stride walks over need no division by the queries
   p.queries = (int)a->queries;
+  if (a->queries == 1) {
+    p.kvs[1] = p.kvs[0];
+    p.krs[1] = p.krs[0];
+    p.queries = 0;
+  } else if (a->batch == 1 || (p.kvs[0] == a->queries * p.kvs[1] && p.krs[0] == a->queries * p.krs[1])) {
+    p.queries = 0;
+  }
   p.half = a->layout == DSA_ROPE_HALF;
   p.factor = a->attention_factor;
   return launch_status(dsa::launch_append_kv(p, static_cast<cudaStream_t>(stream)));

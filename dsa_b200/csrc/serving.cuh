@@ -54,7 +54,8 @@ struct AppendParams {
   uint8_t* cache;               // [rows, 656] (FP8 cache) or null
   long long kvs[2], krs[2];     // strides in elements: batch, query
   long long tokens, rows;
-  int queries, half;
+  int queries;                  // 0: token t lies at t * strides[1]
+  int half;
   float factor;
 };
 cudaError_t launch_append_kv(const AppendParams& p, cudaStream_t stream);

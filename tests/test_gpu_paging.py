@@ -209,6 +209,45 @@ def test_append_signed_zeros_and_mixed_blocks(cuda_lib):
     assert torch.equal(cache[..., :512][~nan], want[..., :512][~nan]) and torch.equal(cache[..., 512:], want[..., 512:])
 
 
+def test_append_every_mantissa(cuda_lib):
+    """Bit for bit the host writer's rows for all pairs of a value's and a maximum's BF16 mantissa, at several exponents:
+    scales and quotients are the rounded quotients, ties of the FP8 rounding among them."""
+    top = (128 + torch.arange(128)).float().reshape(128, 1)                  # a block's maximum
+    low = (128 + torch.arange(128)).float().reshape(1, 128) * 0.5            # 64 .. 127.5: below every maximum
+    blocks = torch.cat([low * 2.0 ** -(torch.arange(128) % 9).float() * (1 - 2 * (torch.arange(128) % 2)), low, low / 16])
+    blocks = torch.stack([b.expand(128, 128).clone() for b in blocks])       # [3, 128 maxima, 128 values]
+    blocks[:, :, 0] = top.squeeze(1)
+    blocks = torch.cat([blocks, blocks.roll(1, -1)])                         # mantissa 0 meets every maximum by its double
+    kv = torch.stack([blocks, blocks * 2.0 ** -50, blocks * 2.0 ** 40]).reshape(1, -1, 1, 512).bfloat16().cuda()
+    assert torch.equal(kv[0, :192].float().cpu().reshape(blocks.shape), blocks)
+    tokens = kv.shape[1]
+    kr = torch.zeros((1, tokens, 1, 64), dtype=torch.bfloat16, device="cuda")
+    slots = torch.arange(tokens, dtype=torch.int32, device="cuda").reshape(1, tokens)
+    cache = torch.zeros((1, tokens, 1, 656), dtype=torch.uint8, device="cuda")
+    dsa_b200.append_kv_fp8(kv, kr, slots, cache)
+    assert torch.equal(cache, dsa_b200.quantize_kv_fp8(kv.cpu(), kr.cpu()).cuda())
+
+
+@pytest.mark.parametrize("batch,queries", [(3, 5), (5, 1), (1, 6), (2, 4)])
+@pytest.mark.parametrize("gap", ["none", "kv", "rope", "both"])
+def test_append_batch_strides(cuda_lib, batch, queries, gap):
+    """Rows of a batch with and without a gap behind each row's tokens, for the latent and the rope values apart."""
+    kv, kr = _tokens(batch, queries, 21)
+    slots = torch.randperm(batch * queries + 7, device="cuda")[:batch * queries].int().reshape(batch, queries)
+    pos = torch.randint(0, 9999, (batch, queries), dtype=torch.int32, device="cuda")
+    kw = dict(positions=pos, inv_freq=dsa_b200.rotary_frequencies(64, device="cuda"))
+    pad = lambda t: torch.cat([t, torch.full_like(t, 9.0)], 1)[:, :queries]
+    got, want = [], []
+    for out, x, y in ((want, kv, kr), (got, pad(kv) if gap in ("kv", "both") else kv, pad(kr) if gap in ("rope", "both") else kr)):
+        for n, dtype in ((512, torch.bfloat16), (64, torch.bfloat16), (656, torch.uint8)):
+            out.append(torch.zeros((batch * queries + 7, 1, 1, n), dtype=dtype, device="cuda"))
+        dsa_b200.append_kv(x, y, slots, *out[:2], **kw)
+        dsa_b200.append_kv_fp8(x, y, slots, out[2], **kw)
+    to = slots.flatten().long()
+    assert torch.equal(want[0][to], kv.reshape(-1, 1, 1, 512))
+    assert all(torch.equal(g, w) for g, w in zip(got, want))
+
+
 def test_append_far_rows(cuda_lib):
     """Rows behind 2^31 elements of the BF16 cache and 2^31 bytes of the FP8 cache; the rows around them stay."""
     kv, kr = _tokens(1, 2, 10)
