@@ -44,25 +44,68 @@ struct PrefixPlan {
 // and a read of 2 KB a row, about 5 TB/s, and the join ~0.3 us a part (96 rows
 // over 1000 keys: 8 splits 17.9 us, 16 splits 20.6). A tile of 64 keys takes a cluster of one row tile ~1,400
 // cycles and one of two ~1,200; the latter leaves half a cluster idle when the
-// row tiles are odd. Returns the estimated time.
-double prefix_split(int64_t row_tiles, int64_t keys, int group, int* split) {
+// row tiles are odd.
+struct PrefixEstimate {
+  double us, kernel_us;  // with and without what the partials cost afterwards
+  int split;
+  int64_t sms;           // that hold a CTA of the kernel
+};
+PrefixEstimate prefix_split(int64_t row_tiles, int64_t keys, int group) {
   int clusters = dsa::prefix_max_clusters(group);
   if (clusters <= 0) clusters = 74 / group;
   const int64_t tiles = (keys + 63) / 64, sets = (row_tiles + group - 1) / group;
   const double tile_us = group == 1 ? 0.85 : 0.73;
-  double best = 0;
-  *split = 1;
+  PrefixEstimate best{0, 0, 1, 0};
   // more than four waves of items never pay
   for (int s = 1; s <= 128 && s <= tiles && (s == 1 || sets * s <= 4 * (int64_t)clusters); ++s) {
     const int64_t waves = (sets * s + clusters - 1) / clusters;
-    const double us = tile_us * (double)waves * (double)((tiles + s - 1) / s + 12) +
-                      (s > 1 ? 1.0 + 0.3 * s + (double)row_tiles * s * 128 * 4096 / 5e6 : 0.0);
-    if (s == 1 || us < best) {
-      best = us;
-      *split = s;
-    }
+    const double kernel = tile_us * (double)waves * (double)((tiles + s - 1) / s + 12);
+    const double us = kernel + (s > 1 ? 1.0 + 0.3 * s + (double)row_tiles * s * 128 * 4096 / 5e6 : 0.0);
+    if (s == 1 || us < best.us) best = {us, kernel, s, 2 * group * (sets * s < clusters ? sets * s : (int64_t)clusters)};
   }
   return best;
+}
+
+// Splits of the own keys, which run beside the prefix kernel: `idle` places
+// (CTAs or pairs) are free from the start, `busy` ones once that kernel ends,
+// and items of one length d go to whichever is free, so what counts is how many
+// rounds remain when the prefix is done. The end is the first time by which the
+// places have run all items; each split adds its partials. A kernel time 5 %
+// off either way counts as likely, so that a choice does not hang on an item
+// that just fits. Times in us, fitted to thirteen (stream) and ten (pair)
+// shapes, within 1.5 % of the best split on average. Against one wave of splits
+// for all places: 64 queries x 16 heads, 32768 + 2048 keys 107 -> 102; 200 x 16,
+// 4096 + 2048 177 -> 144; 8 x 128, 32768 + 2048 103 -> 70 (all of them beside).
+int own_splits(int64_t items, int64_t rows, int64_t tiles, bool pair, int64_t idle, int64_t busy, double prefix_us) {
+  const double item_us = pair ? 9.5 : 6, tile_us = pair ? 0.88 : 1.8, late_us = pair ? 2 : 10;
+  const double part_us = (pair ? 0.2 : 0.5) + (double)rows * 4096 / (pair ? 2.5e6 : 5e6);
+  int split = 1;
+  double best = 0;
+  for (int s = 1; s <= 16 && (s == 1 || s <= tiles / 2); ++s) {
+    const double d = item_us + tile_us * (double)((tiles + s - 1) / s), n = (double)items * s;
+    double us = part_us * s;
+    for (const double f : {0.95, 1.0, 1.05}) {
+      const double t0 = prefix_us * f + late_us;
+      const auto done = [&](double t) {
+        return (double)idle * std::floor(t / d + 1e-6) + (t < t0 ? 0.0 : (double)busy * std::floor((t - t0) / d + 1e-6));
+      };
+      // places that never pause would be through by `low`; an item ends at a multiple of d
+      const double alone = idle > 0 ? n * d / (double)idle : t0 + 1;
+      const double low = alone <= t0 ? alone : (n * d + (double)busy * t0) / (double)(idle + busy);
+      double end = 1e300;
+      for (const double from : {0.0, t0}) {
+        double k = std::fmax(0.0, std::floor((low - from) / d));
+        while (done(from + k * d) < n) k += 1;
+        end = std::fmin(end, from + k * d);
+      }
+      us += std::fmax(end, t0) / 3;
+    }
+    if (s == 1 || us < best) {
+      best = us;
+      split = s;
+    }
+  }
+  return split;
 }
 
 bool plan_prefix(const dsa_fwd_args_t* a, const dsa_prefix_kv_t* px, PrefixPlan* plan) {
@@ -75,24 +118,20 @@ bool plan_prefix(const dsa_fwd_args_t* a, const dsa_prefix_kv_t* px, PrefixPlan*
   if (!product_ok(plan->tokens, a->heads, 1LL << 37)) return false;
   plan->rows = plan->tokens * a->heads;
   plan->row_tiles = (plan->rows + 127) / 128;
-  int split1 = 1, split2 = 1;
-  const double one = prefix_split(plan->row_tiles, px->rows, 1, &split1), two = prefix_split(plan->row_tiles, px->rows, 2, &split2);
-  plan->group = two < one ? 2 : 1;
-  plan->split = plan->group == 2 ? split2 : split1;
+  const PrefixEstimate one = prefix_split(plan->row_tiles, px->rows, 1), two = prefix_split(plan->row_tiles, px->rows, 2);
+  const PrefixEstimate& taken = two.us < one.us ? two : one;
+  plan->group = two.us < one.us ? 2 : 1;
+  plan->split = taken.split;
   if ((plan->row_tiles + 1) * plan->split > kMaxInt / 2) return false;
   plan->own_split = 0;
   if (own) {
-    // own keys: one wave of the pair (H = 128) or stream family's CTAs, two
-    // tiles of 32 keys at least per split; items of at most 64 tiles, which
-    // fill the SMs that the prefix leaves or frees
-    const int64_t tiles = (a->topk + 31) / 32;
-    int64_t ctas = a->heads == 128 ? dsa::pair_max_ctas() / 2 : dsa::stream_max_ctas();
-    if (ctas <= 0) ctas = a->heads == 128 ? 74 : 296;
-    int64_t s = ctas / (a->heads == 128 ? plan->tokens : plan->tokens * (a->heads / 16));
-    if (s < (tiles + 63) / 64) s = (tiles + 63) / 64;
-    if (s > tiles / 2) s = tiles / 2;
-    if (s > 16) s = 16;
-    plan->own_split = (int)(s < 1 ? 1 : s);
+    // own keys: pairs of CTAs (H = 128) or the stream family's CTAs, a 16-head group each
+    const bool pair = a->heads == 128;
+    int64_t places = pair ? dsa::pair_max_ctas() / 2 : dsa::stream_max_ctas();
+    if (places <= 0) places = pair ? 74 : 296;
+    const int64_t sms = 148, busy = places * (taken.sms < sms ? taken.sms : sms) / sms;
+    plan->own_split = own_splits(pair ? plan->tokens : plan->tokens * (a->heads / 16), plan->rows, (a->topk + 31) / 32, pair,
+                                 places - busy, busy, taken.kernel_us);
   }
   plan->direct = !own && plan->split == 1;
   plan->num = plan->max = plan->sum = plan->own_num = plan->own_max = plan->own_sum = plan->total = 0;
