@@ -87,6 +87,11 @@ def _check_rope(positions, inv_freq, layout, attention_factor, lead, index):
     return number
 
 
+def _rows_like(x):
+    """A contiguous tensor of the shape of ``x`` (half the host time of ``torch.empty``)."""
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
+
+
 def _launch(x, positions, inv_freq, out, number, start, factor, inverse):
     p0, p1 = positions.stride()
     if x.dim() == 4:
@@ -109,11 +114,11 @@ class _Rotary(torch.autograd.Function):
     """The rotation is linear with an orthogonal matrix times the factor: its gradient is the inverse rotation."""
 
     @staticmethod
-    def forward(ctx, x, positions, inv_freq, number, start, factor, inverse):
+    def forward(ctx, x, turn):  # one argument beside x: every further one costs the engine host time
+        positions, inv_freq, *how = turn
         ctx.save_for_backward(positions, inv_freq)
-        ctx.how = (number, start, factor, inverse)
-        return _launch(x, positions, inv_freq, torch.empty(x.shape, dtype=x.dtype, device=x.device), number, start,
-                       factor, inverse)
+        ctx.how = how
+        return _launch(x, positions, inv_freq, _rows_like(x), *how)
 
     @staticmethod
     def backward(ctx, grad):
@@ -122,11 +127,8 @@ class _Rotary(torch.autograd.Function):
         if grad.stride(-1) != 1:
             grad = grad.contiguous()
         if torch.is_grad_enabled():  # a graph of the gradient is wanted
-            gx = _Rotary.apply(grad, positions, inv_freq, number, start, factor, not inverse)
-        else:
-            gx = _launch(grad, positions, inv_freq, torch.empty(grad.shape, dtype=grad.dtype, device=grad.device), number,
-                         start, factor, not inverse)
-        return gx, None, None, None, None, None, None
+            return _Rotary.apply(grad, (positions, inv_freq, number, start, factor, not inverse)), None
+        return _launch(grad, positions, inv_freq, _rows_like(grad), number, start, factor, not inverse), None
 
 
 def rotary(x, positions, inv_freq, *, layout="interleaved", start=0, attention_factor=1.0, inverse=False, out=None):
@@ -168,9 +170,8 @@ def rotary(x, positions, inv_freq, *, layout="interleaved", start=0, attention_f
     inverse = bool(inverse)
     if out is None:
         if x.requires_grad and torch.is_grad_enabled():
-            return _Rotary.apply(x, positions, inv_freq, number, start, attention_factor, inverse)
-        return _launch(x, positions, inv_freq, torch.empty(shape, dtype=x.dtype, device=device), number, start,
-                       attention_factor, inverse)
+            return _Rotary.apply(x, (positions, inv_freq, number, start, attention_factor, inverse))
+        return _launch(x, positions, inv_freq, _rows_like(x), number, start, attention_factor, inverse)
     if out.shape != x.shape or out.dtype != x.dtype or out.device != device or out.stride(-1) != 1 or _overlaps_itself(out):
         raise ValueError("out must have the shape, type and device of x and rows that do not overlap")
     if torch.is_grad_enabled() and (x.requires_grad or out.requires_grad):
