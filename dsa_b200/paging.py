@@ -71,15 +71,14 @@ def plan_pages(block_table, cached_lens, new_lens, free_blocks, free_count, bloc
             or batch * max_blocks > 0x7fffffff):
         raise ValueError("a table, the page pool or the step holds more than 2^31 - 1 entries")
     # few allocations and views: they cost more host time than the kernels take
-    positions, lengths, slots = torch.empty((3, batch, queries), dtype=int32, device=device).unbind(0)
+    positions, lengths, slots = block_table.new_empty((3, batch, queries)).unbind(0)
     words = 4 * batch + 4
     if inplace:
         table, lens, stack, count = block_table, cached_lens, free_blocks, free_count
-        work, missing = torch.empty(words + 1, dtype=int32, device=device).split_with_sizes((words, 1))
+        work, missing = block_table.new_empty(words + 1).split_with_sizes((words, 1))
     else:
         table, stack = torch.empty_like(block_table), torch.empty_like(free_blocks)
-        work, missing, count, lens = torch.empty(words + 2 + batch, dtype=int32, device=device).split_with_sizes(
-            (words, 1, 1, batch))
+        work, missing, count, lens = block_table.new_empty(words + 2 + batch).split_with_sizes((words, 1, 1, batch))
     api.enqueue("dsa_plan_pages", _native.PlanPagesArgs(
         block_table.data_ptr(), cached_lens.data_ptr(), new_lens.data_ptr(), free_blocks.data_ptr(),
         free_count.data_ptr(), None if reset is None else reset.data_ptr(), table.data_ptr(), lens.data_ptr(),

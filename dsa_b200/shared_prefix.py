@@ -78,7 +78,7 @@ def forward_shared_prefix(q, prefix_kv, q_rope, prefix_k_rope, kv=None, k_rope=N
     if prefix > 1 << 26 or batch * queries > 0x7fffffff or batch * length > 0x7fffffff:
         raise ValueError("the prefix holds more than 2^26 rows, or the batch more than 2^31 - 1 queries or keys")
     output = torch.empty_like(q)
-    maximum = torch.empty((batch, 1, queries, heads), device=device, dtype=torch.float32)
+    maximum = q.new_empty((batch, 1, queries, heads), dtype=torch.float32)
     denominator = torch.empty_like(maximum)
     px = _native.PrefixKv(prefix_kv.data_ptr(), prefix_k_rope.data_ptr(),
                           None if prefix_len is None else prefix_len.data_ptr(), prefix)
