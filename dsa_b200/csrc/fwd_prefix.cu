@@ -826,8 +826,10 @@ __global__ void __launch_bounds__(kPxThreads, 1) fwd_prefix_kernel(const PrefixP
 // memory. Bound by the partials' 2 KB a row and part, and with few rows by
 // latency: a thread's first four parts are under way before the weights are
 // known (8192 rows of 3 parts 20 -> 15 us from DRAM; eight in flight cost
-// occupancy, 21 us). A part of weight 0 counts as 0 whatever its numerator
-// holds (nothing is written there when it has no keys).
+// occupancy, 21 us). A part without keys (sum 0) is left out: nothing is written
+// to its numerator then. Every other part counts, whatever its weight: the
+// maximum of a part whose scores are all NaN says nothing, and its NaN sum has
+// to reach the row.
 constexpr int kJoinWarps = 8;
 constexpr int kJoinMaxParts = 160;
 
@@ -879,8 +881,8 @@ __global__ void __launch_bounds__(32 * kJoinWarps) prefix_join_kernel(const Join
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const float2 ml = i0 + j < n ? stats[i0 + j][lane] : make_float2(0.f, 0.f);
-      const float w = ml.y != 0.f ? expf(ml.x - top) : 0.f;
-      if (w != 0.f) {
+      if (ml.y != 0.f) {
+        const float w = expf(ml.x - top);
         total = fmaf(w, ml.y, total);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {

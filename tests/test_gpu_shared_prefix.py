@@ -159,3 +159,27 @@ def test_other_stream_and_unequal_calls_at_once(cuda_lib):
     torch.cuda.synchronize()
     _check(first, a, 3000)
     _check(second, b, 1500)
+
+
+@pytest.mark.parametrize("heads", [16, 48, 128])
+@pytest.mark.parametrize("where", ["own", "prefix", "one own key far below"])
+def test_nan_in_live_keys(cuda_lib, heads, where):
+    """A NaN score makes its row NaN whichever part of the keys it lies in; the rows without one stay as they are."""
+    args = _make(2, 2, heads, 4097, 300, 77, seed=1)
+    q, pk, qr, pr, kv, kr, ids = args
+    ids[:, :, :, 0] = 7
+    if where == "own":
+        kv[1] = float("nan")  # every key of the part: it has no maximum
+    elif where == "prefix":
+        pk[0, :2048] = float("nan")
+    else:  # row (1, 0, 0): 8 |q|^2 / 24 = 8 * 576 / 24 ~ 192 for its prefix key, 0 for its own keys: e^-192 is 0 in FP32
+        kv[1], kr[1] = 0, 0
+        kr[1, 7] = float("nan")
+        pk[0, 9, 0], pr[0, 9, 0] = q[1, 0, 0] * 8, qr[1, 0, 0] * 8
+    got = dsa_b200.forward_shared_prefix(*args)
+    out, _, total = got
+    assert bool(out[1].isnan().all()) and bool(total[1].isnan().all())
+    if where == "prefix":
+        assert bool(out.isnan().all()) and bool(total.isnan().all())
+    else:
+        _check([t[:1] for t in got], (q[:1], pk, qr[:1], pr, kv[:1], kr[:1], ids[:1]), 4097)
