@@ -900,7 +900,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) prefix_join_kernel(const Join
       make_uint4(pack_bf16x2(acc[0] * rl, acc[1] * rl), pack_bf16x2(acc[2] * rl, acc[3] * rl),
                  pack_bf16x2(acc[4] * rl, acc[5] * rl), pack_bf16x2(acc[6] * rl, acc[7] * rl));
   if (col == 0) {
-    p.out_max[r] = total != 0.f ? top : -INFINITY;
+    p.out_max[r] = total > 0.f ? top : -INFINITY;  // -inf beside a NaN sum, as final_max gives
     p.out_sum[r] = total;
   }
 }

@@ -33,8 +33,9 @@ def forward_shared_prefix(q, prefix_kv, q_rope, prefix_k_rope, kv=None, k_rope=N
     Returns ``(output, softmax_max, softmax_sum)`` as ``forward`` does, over
     both sets of keys: indices outside ``[0, L)`` are masked, duplicates keep
     their repeated weight, a row without any key gets output 0, maximum -inf
-    and sum 0. Asynchronous on the current stream; partials are FP32, in
-    pieces of whole queries that keep them under ``WORKSPACE_BUDGET`` bytes.
+    and sum 0, one with a NaN score NaN, -inf and NaN. Asynchronous on the
+    current stream; partials are FP32, in pieces of whole queries that keep
+    them under ``WORKSPACE_BUDGET`` bytes.
     """
     shape = q.shape
     if len(shape) != 4 or prefix_kv.dim() != 4:

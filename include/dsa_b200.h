@@ -348,8 +348,9 @@ DSA_B200_API uint64_t dsa_fwd_prefix_workspace_bytes(const dsa_fwd_args_t* args,
  * are NULL / 0 for attention over the prefix alone. The prefix is read once
  * per 128 (query, head) rows and split over the GPU; partials are joined in
  * FP32. launch.family is AUTO. A row without any key gets output 0,
- * softmax_max -inf, softmax_sum 0; prefix rows at and past the length do not
- * matter, whatever they hold. Returns a dsa_status_t. */
+ * softmax_max -inf, softmax_sum 0, one with a NaN score NaN, -inf and NaN;
+ * prefix rows at and past the length do not matter, whatever they hold.
+ * Returns a dsa_status_t. */
 DSA_B200_API int dsa_sparse_mla_fwd_prefix(const dsa_fwd_args_t* args, const dsa_prefix_kv_t* prefix, void* stream);
 
 /* Number of kernels the last successful dsa_sparse_mla_fwd on this host

@@ -183,3 +183,22 @@ def test_nan_in_live_keys(cuda_lib, heads, where):
         assert bool(out.isnan().all()) and bool(total.isnan().all())
     else:
         _check([t[:1] for t in got], (q[:1], pk, qr[:1], pr, kv[:1], kr[:1], ids[:1]), 4097)
+
+
+@pytest.mark.parametrize("batch,heads,prefix,topk", [(160, 128, 130, 0), (2, 128, 3000, 0), (2, 16, 500, 40), (2, 128, 500, 40)])
+def test_statistics_of_nan_rows(cuda_lib, batch, heads, prefix, topk):
+    """Maximum -inf and sum NaN, as ``forward`` gives, whether or not the kernel writes the output itself and whatever the
+    other parts hold."""
+    args = _make(batch, 1, heads, prefix, 90, topk, seed=2)
+    args[0][0, 0, 5] = float("nan")
+    _, top, total = dsa_b200.forward_shared_prefix(*args)
+    row = torch.zeros_like(top, dtype=torch.bool)
+    row[0, 0, 0, 5] = True
+    assert torch.equal(total.isnan(), row) and torch.equal(top == -float("inf"), row)
+    args[1][0, 3] = float("nan")
+    _, top, total = dsa_b200.forward_shared_prefix(*args)
+    assert bool(total.isnan().all()) and bool((top == -float("inf")).all())
+    if topk:
+        q, _, qr, _, kv, kr, ids = args
+        _, top, total = dsa_b200.forward(q, kv, qr, kr, ids)
+        assert torch.equal(total.isnan(), row) and torch.equal(top == -float("inf"), row)
