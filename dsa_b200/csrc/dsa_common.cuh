@@ -76,8 +76,10 @@ struct FwdParams {
   int wait_test;
   // The launch may run beside the kernel before it in the stream, on which
   // nothing here depends, one item per cluster or CTA; every split's partials
-  // are kept (split 1 too), and it ends after that kernel, for which its last
-  // CTAs wait (pair and stream families).
+  // are kept (split 1 too), the values of masked keys are zeros (weight 0 times
+  // a NaN of the row that a masked index is clamped to would not be 0), and it
+  // ends after that kernel, for which its last CTAs wait (pair and stream
+  // families).
   int beside_previous;
 };
 
@@ -124,6 +126,10 @@ __device__ __forceinline__ uint32_t smem_u32(const void* p) {
 
 __device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src) : "memory");
+}
+// The same, or 16 zero bytes (src is not read).
+__device__ __forceinline__ void cp_async_16_or_zero(uint32_t dst, const void* src, bool zero) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(zero ? 0u : 16u) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() {
   asm volatile("cp.async.commit_group;\n" ::: "memory");

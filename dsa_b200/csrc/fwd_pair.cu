@@ -278,6 +278,8 @@ __device__ __forceinline__ void mma_commit_mc(uint32_t bar, uint16_t cta_mask) {
 
 // 16-byte cp.async of 32 indexed rows into a swizzled K-major stage:
 // `nblk` 64-dim blocks of the latent row (+ the rope block when `rope`).
+// kZero: a negative row gives a latent row of zeros.
+template <bool kZero = false>
 __device__ __forceinline__ void gather_rows(uint32_t stage, const __nv_bfloat16* kv_b, const __nv_bfloat16* kr_b,
                                             int row, int lane, bool rope, int32_t* status) {
   const int j8 = lane & 7;
@@ -289,10 +291,14 @@ __device__ __forceinline__ void gather_rows(uint32_t stage, const __nv_bfloat16*
     const uint32_t dst = checked_smem(
         stage + (uint32_t)(k >> 3) * 1024u + (uint32_t)(k & 7) * 128u + (uint32_t)((j8 ^ (k & 7)) * 16),
         (rope ? 8u : 7u) * kBlk + 16u, stage, rope ? kKStage : kVStage, status);
-    const __nv_bfloat16* src = kv_b + (size_t)rk * kDimLatent + j8 * 8;
+    const int at = kZero ? max(rk, 0) : rk;
+    const __nv_bfloat16* src = kv_b + (size_t)at * kDimLatent + j8 * 8;
 #pragma unroll
-    for (int kb = 0; kb < 8; ++kb) cp_async_16(dst + kb * kBlk, src + kb * 64);
-    if (rope) cp_async_16(dst + 8 * kBlk, kr_b + (size_t)rk * kDimRope + j8 * 8);
+    for (int kb = 0; kb < 8; ++kb) {
+      if constexpr (kZero) cp_async_16_or_zero(dst + kb * kBlk, src + kb * 64, rk < 0);
+      else cp_async_16(dst + kb * kBlk, src + kb * 64);
+    }
+    if (rope) cp_async_16(dst + 8 * kBlk, kr_b + (size_t)at * kDimRope + j8 * 8);
   }
 }
 
@@ -795,9 +801,10 @@ __global__ void __launch_bounds__(kPrThreads, 1) fwd_pair_kernel(const FwdParams
       uint32_t n = 0;
       while (cur.item < n_items) {
         if (n > 0 && !(ok = wait_warp(bar(kVFree0 + s), (n - 1) & 1u, abort_flag))) break;
-        const int row = checked_index(pcursor_row(p, idx_cur, L), L, p.status);  // invalid rows get P = 0
+        int row = checked_index(pcursor_row(p, idx_cur, L), L, p.status);  // invalid rows get P = 0
+        if (kBeside && (idx_cur < 0 || idx_cur >= L)) row = -1;            // and V = 0
         const int gb = checked_index(cur.w.batch, p.batch, p.status);
-        gather_rows(stage, p.kv + (size_t)gb * L * kDimLatent, nullptr, row, lane, false, p.status);
+        gather_rows<kBeside>(stage, p.kv + (size_t)gb * L * kDimLatent, nullptr, row, lane, false, p.status);
         cp_async_commit();
         const int idx_nx2 = pcursor_index(p, nx2, n_items, lane);
         cp_async_wait<0>();

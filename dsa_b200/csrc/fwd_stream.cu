@@ -273,7 +273,8 @@ __global__ void __launch_bounds__(kStThreads, 2) fwd_stream_kernel(const FwdPara
         if (!ok) break;
       }
       if ((lane >> 4) == hw) sm.ids[u][lane & 15] = idx_cur;  // validity is judged from the original index
-      const int row = checked_index(min(max(idx_cur, 0), L - 1), L, p.status);
+      int row = checked_index(min(max(idx_cur, 0), L - 1), L, p.status);
+      if (kBeside && (idx_cur < 0 || idx_cur >= L)) row = -1;  // zeros
       const int gb = checked_index(cur.w.batch, p.batch, p.status);
       const __nv_bfloat16* kv_b = p.kv + (size_t)gb * L * kDimLatent;
       const __nv_bfloat16* kr_b = p.k_rope + (size_t)gb * L * kDimRope;
@@ -284,10 +285,17 @@ __global__ void __launch_bounds__(kStThreads, 2) fwd_stream_kernel(const FwdPara
         const int rk = __shfl_sync(0xffffffffu, row, 16 * hw + key);
         const uint32_t dst = checked_smem(unit + (uint32_t)(key * kStRow + j8 * 8) * 2u, 8u * 128u + 16u, unit,
                                           kStUnitBytes, p.status);
-        const __nv_bfloat16* src = kv_b + (size_t)rk * kDimLatent + j8 * 8;
+        if constexpr (kBeside) {
+          const __nv_bfloat16* src = kv_b + (size_t)max(rk, 0) * kDimLatent + j8 * 8;
 #pragma unroll
-        for (int kb = 0; kb < 8; ++kb) cp_async_16(dst + kb * 128u, src + kb * 64);
-        cp_async_16(dst + 8u * 128u, kr_b + (size_t)rk * kDimRope + j8 * 8);
+          for (int kb = 0; kb < 8; ++kb) cp_async_16_or_zero(dst + kb * 128u, src + kb * 64, rk < 0);
+          cp_async_16_or_zero(dst + 8u * 128u, kr_b + (size_t)max(rk, 0) * kDimRope + j8 * 8, rk < 0);
+        } else {
+          const __nv_bfloat16* src = kv_b + (size_t)rk * kDimLatent + j8 * 8;
+#pragma unroll
+          for (int kb = 0; kb < 8; ++kb) cp_async_16(dst + kb * 128u, src + kb * 64);
+          cp_async_16(dst + 8u * 128u, kr_b + (size_t)rk * kDimRope + j8 * 8);
+        }
       }
       cp_async_mbar_arrive_noinc(full0 + 8u * u);
       const int idx_nx2 = st_index(p, nx2, n_items, lane);  // consumed two tiles later

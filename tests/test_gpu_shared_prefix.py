@@ -202,3 +202,18 @@ def test_statistics_of_nan_rows(cuda_lib, batch, heads, prefix, topk):
         q, _, qr, _, kv, kr, ids = args
         _, top, total = dsa_b200.forward(q, kv, qr, kr, ids)
         assert torch.equal(total.isnan(), row) and torch.equal(top == -float("inf"), row)
+
+
+@pytest.mark.parametrize("heads", [16, 48, 128])
+def test_nan_behind_masked_indices(cuda_lib, heads):
+    """Own rows that no valid index names may hold NaN: also the first and the last row, on which masked indices fall
+    (negative ones, those past the end), alone in a tile or beside valid ones."""
+    args = _make(3, 2, heads, 500, 90, 77, seed=3)
+    kv, kr, ids = args[4:]
+    ids[ids == 0], ids[ids == 89] = 1, 88
+    ids[..., 5], ids[..., 6], ids[..., 40:72] = 90, 2 ** 31 - 1, -2 ** 31
+    ids[0, 1, :, 32:] = -1
+    ids[2, 0] = 90
+    for row, value in ((0, float("nan")), (89, float("inf"))):
+        kv[:, row], kr[:, row] = value, value
+    _check(dsa_b200.forward_shared_prefix(*args), args, 500)
