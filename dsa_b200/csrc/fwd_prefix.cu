@@ -31,7 +31,11 @@
 // 8 KB boxes could not keep a tile's pace.
 //
 // P rounds the weights to BF16 for the MMA; the row sum adds them before the
-// rounding, in FP32 (as every other family here).
+// rounding, in FP32 (as every other family here). A score is 36 accumulations
+// of the MMA, each cut to FP32: on random data it ends 5.6e-7 of itself too
+// near to zero on average (so does the pair family's), and is exact where the
+// products' sums are. Nothing corrects for it: the loss depends on the data,
+// and the own keys' scores, which share the softmax, lose theirs alike.
 //
 // Roles (12 warps; the MMAs of a pair are issued by its first CTA): score CTA
 // 0 TMA, 1 and 3 QK issuers of the even and the odd tiles, in turn (an issuer
@@ -71,13 +75,6 @@ constexpr int kSoftWarp0 = 4;
 constexpr int kEpiWarps = 8;
 constexpr uint32_t kReqEnd = 0xffffffffu;
 constexpr uint32_t kTmemCols = 512, kTmemQ = 0, kTmemS = 288, kTmemO = 0;
-// The MMA cuts each of a score's 36 accumulations to FP32 instead of rounding
-// it: half a unit in the last place is lost on average, 2^-25 to 2^-24 of a sum
-// that has grown half way, together 36 / 2 * 2^-24.8 = 6e-7 of the score (5.6e-7
-// measured, always towards zero). Scaling by 1 + 5.6e-7 takes the mean error of
-// softmax_max from -5.6e-7 to below 1e-7 relative and with it that of softmax_sum,
-// which is relative to the maximum, from 1.8e-6 to 5e-7.
-constexpr double kCutBias = 5.6e-7;
 
 // Sizes and barriers that depend on the CTAs of a pair. "Leader": the barrier
 // of the pair's first CTA is used by both.
@@ -998,10 +995,7 @@ cudaError_t launch(const PrefixParams& p, const void* kv, const void* k_rope, cu
 int prefix_max_clusters(int group) { return group == 2 ? max_clusters<2>() : max_clusters<1>(); }
 
 cudaError_t launch_fwd_prefix(const PrefixParams& p, const void* kv, const void* k_rope, cudaStream_t stream) {
-  PrefixParams scaled = p;
-  scaled.scale_div = (float)(p.scale_div * (1.0 - kCutBias));
-  scaled.scale_log2 = (float)(p.scale_log2 * (1.0 + kCutBias));
-  return p.group == 2 ? launch<2>(scaled, kv, k_rope, stream) : launch<1>(scaled, kv, k_rope, stream);
+  return p.group == 2 ? launch<2>(p, kv, k_rope, stream) : launch<1>(p, kv, k_rope, stream);
 }
 
 cudaError_t launch_prefix_join(const JoinParams& p, cudaStream_t stream) {

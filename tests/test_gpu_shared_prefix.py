@@ -217,3 +217,36 @@ def test_nan_behind_masked_indices(cuda_lib, heads):
     for row, value in ((0, float("nan")), (89, float("inf"))):
         kv[:, row], kr[:, row] = value, value
     _check(dsa_b200.forward_shared_prefix(*args), args, 500)
+
+
+@pytest.mark.parametrize("batch,heads,prefix,topk", [
+    (2, 16, 700, 0), (2, 16, 700, 40), (2, 128, 700, 40), (3, 48, 3000, 33), (160, 128, 130, 0), (70, 128, 65, 0)])
+def test_exact_scores(cuda_lib, batch, heads, prefix, topk):
+    """Small whole numbers, whose products and sums are exact in FP32 in any order: the maximum is the largest score's
+    rounded quotient by 24, to the last bit, whichever set of keys it lies in. A key that is in both sets has one weight:
+    with every prefix key among the own ones the sum doubles and the output stays, up to the exponentials' rounding."""
+    g = torch.Generator(device="cuda").manual_seed(4)
+
+    def r(*shape):
+        return torch.randint(-1, 2, shape, generator=g, device="cuda").bfloat16()
+
+    q, pk, qr, pr = r(batch, 1, heads, 512), r(1, prefix, 1, 512), r(batch, 1, heads, 64), r(1, prefix, 1, 64)
+    own = [None, None, None]
+    if topk:
+        ids = torch.randint(0, 90, (batch, 1, 1, topk), generator=g, device="cuda", dtype=torch.int32)
+        own = [r(batch, 90, 1, 512), r(batch, 90, 1, 64), ids]
+    args = (q, pk, qr, pr, *own)
+    got = dsa_b200.forward_shared_prefix(*args)
+    _, top, total, _, _ = _reference(*args, prefix, 1.0)  # whole scores
+    assert torch.equal(got[1][:, 0].cpu(), top.float().cpu() / 24.0)
+    _, _, total, _, _ = _reference(*args, prefix, 1 / 24)
+    # |score| < 8 (576 products of -1, 0, 1: a standard deviation of 16 / 24): exponents below 12 of FP32 rounding, 2^-20,
+    # the exponential's 2^-22 and the sum's
+    assert bool(((got[2][:, 0].double() - total).abs() <= total * 2.0 ** -18).all())
+    if topk:
+        every = torch.arange(prefix, device="cuda", dtype=torch.int32).expand(batch, 1, 1, prefix).contiguous()
+        both = dsa_b200.forward_shared_prefix(q, pk, qr, pr, pk.expand(batch, -1, -1, -1).contiguous(),
+                                              pr.expand(batch, -1, -1, -1).contiguous(), every)
+        alone = dsa_b200.forward_shared_prefix(q, pk, qr, pr)
+        assert torch.equal(both[1], alone[1])
+        assert bool(((both[2] / 2 - alone[2]).abs() <= alone[2] * 2.0 ** -17).all())
