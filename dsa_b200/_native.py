@@ -52,6 +52,7 @@ EXPORTS = (
     "dsa_plan_pages",
     "dsa_append_kv",
     "dsa_fwd_prefix_workspace_bytes",
+    "dsa_fwd_prefix_plan",
     "dsa_sparse_mla_fwd_prefix",
 )
 
@@ -206,6 +207,8 @@ def _bind(lib):
     lib.dsa_indexer_topk.argtypes = [ctypes.POINTER(IndexerArgs), ctypes.c_void_p]
     lib.dsa_fwd_prefix_workspace_bytes.restype = ctypes.c_uint64
     lib.dsa_fwd_prefix_workspace_bytes.argtypes = [ctypes.POINTER(FwdArgs), ctypes.POINTER(PrefixKv)]
+    lib.dsa_fwd_prefix_plan.restype = ctypes.c_int
+    lib.dsa_fwd_prefix_plan.argtypes = [ctypes.POINTER(FwdArgs), ctypes.POINTER(PrefixKv), ctypes.POINTER(ctypes.c_int32)]
     lib.dsa_sparse_mla_fwd_prefix.restype = ctypes.c_int
     lib.dsa_sparse_mla_fwd_prefix.argtypes = [ctypes.POINTER(FwdArgs), ctypes.POINTER(PrefixKv), ctypes.c_void_p]
     lib.dsa_rotary.restype = ctypes.c_int

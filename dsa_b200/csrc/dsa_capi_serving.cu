@@ -277,6 +277,15 @@ uint64_t dsa_fwd_prefix_workspace_bytes(const dsa_fwd_args_t* a, const dsa_prefi
   return plan_prefix(a, px, &plan) ? plan.total : 0;
 }
 
+int dsa_fwd_prefix_plan(const dsa_fwd_args_t* a, const dsa_prefix_kv_t* px, int32_t out[3]) {
+  PrefixPlan plan;
+  if (out == nullptr || !plan_prefix(a, px, &plan)) return DSA_STATUS_BAD_ARGUMENT;
+  out[0] = plan.group;
+  out[1] = plan.split;
+  out[2] = plan.own_split;
+  return DSA_STATUS_OK;
+}
+
 int dsa_sparse_mla_fwd_prefix(const dsa_fwd_args_t* a, const dsa_prefix_kv_t* px, void* stream) {
   PrefixPlan plan;
   if (!plan_prefix(a, px, &plan)) return DSA_STATUS_BAD_ARGUMENT;

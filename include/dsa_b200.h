@@ -342,6 +342,12 @@ typedef struct dsa_prefix_kv {
  * where none is needed. */
 DSA_B200_API uint64_t dsa_fwd_prefix_workspace_bytes(const dsa_fwd_args_t* args, const dsa_prefix_kv_t* prefix);
 
+/* What dsa_sparse_mla_fwd_prefix launches for these sizes on the current
+ * device: row tiles per item (1 or 2: which kernel runs), key splits of the
+ * prefix and of the own keys (0 without own keys). Needs no pointers in args.
+ * Returns a dsa_status_t. */
+DSA_B200_API int dsa_fwd_prefix_plan(const dsa_fwd_args_t* args, const dsa_prefix_kv_t* prefix, int32_t plan[3]);
+
 /* Forward of every query over the prefix keys and its own selected keys, as
  * one softmax: q, q_rope, output and statistics as for dsa_sparse_mla_fwd;
  * kv, k_rope, indices, length and topk describe each batch row's own keys, or

@@ -9,11 +9,13 @@ once more to BF16:
   |out - ref| <= W (2^-8 + 5 D + 2^-18) + 2^-8 |ref|   (2^-18: exponentials, joins)
   |max - ref| <= D + 2^-22 |ref|,  |sum - ref| <= ref (3 D + 2^-18)
 """
+import ctypes
+
 import pytest
 import torch
 
 import dsa_b200
-from dsa_b200 import shared_prefix
+from dsa_b200 import _native, shared_prefix
 
 pytestmark = pytest.mark.gpu
 
@@ -250,3 +252,43 @@ def test_exact_scores(cuda_lib, batch, heads, prefix, topk):
         alone = dsa_b200.forward_shared_prefix(q, pk, qr, pr)
         assert torch.equal(both[1], alone[1])
         assert bool(((both[2] / 2 - alone[2]).abs() <= alone[2] * 2.0 ** -17).all())
+
+
+def _plan(args):
+    """(row tiles per item, prefix splits, own splits) of the call."""
+    a, plan = _native.FwdArgs(), (ctypes.c_int32 * 3)()
+    a.batch, a.queries, a.heads = args[0].shape[:3]
+    if args[6] is not None:
+        a.length, a.topk = args[4].shape[1], args[6].shape[-1]
+    assert _native.load().dsa_fwd_prefix_plan(a, _native.PrefixKv(None, None, None, args[1].shape[1]), plan) == 0
+    return tuple(plan)
+
+
+# 74 row tiles fill the clusters of two SMs and overflow those of four; 37 tiles in two splits likewise
+@pytest.mark.parametrize("batch,queries,heads,prefix,split,length,topk", [
+    *((74, 1, 128, n, 1, 0, 0) for n in (1, 63, 64, 65, 128, 130, 1100)), (74, 8, 16, 300, 1, 0, 0),
+    (37, 1, 128, 4097, 2, 0, 0), (37, 1, 128, 8191, 2, 0, 0), (74, 1, 128, 129, 1, 60, 40), (74, 8, 16, 129, 1, 60, 40),
+    (37, 1, 128, 4097, 2, 90, 77), (37, 2, 64, 4100, 2, 90, 77)])
+def test_one_row_tile_per_item(cuda_lib, batch, queries, heads, prefix, split, length, topk):
+    args = _make(batch, queries, heads, prefix, length, topk, seed=prefix)
+    assert _plan(args)[:2] == (1, split)
+    _check(dsa_b200.forward_shared_prefix(*args), args, prefix)
+
+
+def test_two_row_tiles_per_item(cuda_lib):
+    for shape in ((1, 1, 16, 1, 0, 0), (64, 1, 16, 2048, 4096, 512), (160, 1, 128, 130, 0, 0)):  # of test_parity
+        assert _plan(_make(*shape))[0] == 2
+
+
+@pytest.mark.parametrize("batch,prefix,topk", [(74, 300, 0), (37, 4200, 0), (37, 4200, 40)])
+def test_filled_part_of_one_row_tile_per_item(cuda_lib, batch, prefix, topk):
+    """Lengths on every side of a tile's end, none and all of the buffer, NaN and infinities behind the last key."""
+    args = _make(batch, 1, 128, prefix, 90, topk, seed=6)
+    assert _plan(args)[0] == 1
+    if topk:
+        args[6][3] = -1
+    for n in (0, 1, 63, 64, 65, 130, prefix - 1, prefix):
+        pk, pr = args[1].clone(), args[3].clone()
+        pk[0, n:], pr[0, n:] = float("nan"), float("inf")
+        length = torch.tensor([n], dtype=torch.int32, device="cuda")
+        _check(dsa_b200.forward_shared_prefix(args[0], pk, args[2], pr, *args[4:], prefix_len=length), args, n)

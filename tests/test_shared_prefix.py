@@ -55,3 +55,15 @@ def test_workspace_bytes():
         b.batch, b.queries, b.heads = 2, 1, 16
         setattr(b, field, value)
         assert lib.dsa_sparse_mla_fwd_prefix(ctypes.byref(b), ctypes.byref(px), None) == _native.STATUS_BAD_ARGUMENT
+
+
+def test_plan():
+    lib, a, plan = _native.load(), _native.FwdArgs(), (ctypes.c_int32 * 3)()
+    px = _native.PrefixKv(None, None, None, 32768)
+    a.batch, a.queries, a.heads = 64, 1, 16
+    assert lib.dsa_fwd_prefix_plan(a, px, plan) == 0 and plan[0] in (1, 2) and plan[1] > 1 and plan[2] == 0
+    a.length, a.topk = 100, 64
+    assert lib.dsa_fwd_prefix_plan(a, px, plan) == 0 and plan[2] >= 1
+    assert lib.dsa_fwd_prefix_plan(a, px, None) == _native.STATUS_BAD_ARGUMENT
+    a.heads = 24
+    assert lib.dsa_fwd_prefix_plan(a, px, plan) == _native.STATUS_BAD_ARGUMENT
