@@ -16,6 +16,7 @@ import torch
 
 import dsa_b200
 from dsa_b200 import _native, shared_prefix
+from oracle import sparse_mla as oracle
 
 pytestmark = pytest.mark.gpu
 
@@ -292,3 +293,19 @@ def test_filled_part_of_one_row_tile_per_item(cuda_lib, batch, prefix, topk):
         pk[0, n:], pr[0, n:] = float("nan"), float("inf")
         length = torch.tensor([n], dtype=torch.int32, device="cuda")
         _check(dsa_b200.forward_shared_prefix(args[0], pk, args[2], pr, *args[4:], prefix_len=length), args, n)
+
+
+@pytest.mark.parametrize("batch,queries,heads,prefix,length,topk", [
+    (3, 2, 16, 1000, 300, 77), (5, 7, 32, 4097, 50, 33), (9, 1, 128, 700, 2000, 2048), (160, 1, 128, 130, 0, 0),
+    (74, 1, 128, 1100, 0, 0), (37, 1, 128, 4097, 90, 77), (64, 1, 16, 8192, 4096, 512)])
+def test_framework_gate(cuda_lib, batch, queries, heads, prefix, length, topk):
+    """The framework's requirement on the statistics of every forward, 1e-5, which is tighter than the bound above: each of
+    a score's accumulations loses less than 2^-23 of the partial sum, 44 * 2^-23 = 5.2e-6 if that is the final one's size.
+    The output's requirement, 5e-3 of its largest element, is no bound for rounding: an output of 1.4 with W = 0.8 is off
+    by up to 2^-8 (half a BF16 step in [1, 2)) + 0.8 * 2^-8 = 7.03e-3 > 5e-3 * 1.4; _check has the output's."""
+    args = _make(batch, queries, heads, prefix, length, topk, seed=12)
+    got = [t.float().cpu() for t in dsa_b200.forward_shared_prefix(*args)]
+    out, top, total, _, _ = _reference(*args, prefix, 1 / 24)
+    metrics = oracle.accuracy(got, [t.float().cpu() for t in (out, top[:, None], total[:, None])])
+    for name, gate in oracle.ELEMENT_GATES.items():
+        assert metrics[name]["max_normalized"] <= gate and metrics[name]["max_relative"] <= gate, (name, metrics)
