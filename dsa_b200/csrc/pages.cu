@@ -7,7 +7,9 @@
 // the stack of free pages, rows in order; a reset row's old pages are pushed
 // first. Token s of the row is at position c + s and in cache row
 // table[(c + s) / S] * S + (c + s) % S. Without a page left an entry is -1,
-// and so are the slots of its tokens.
+// and so are the slots of its tokens. Such a page stays missing: what its
+// earlier tokens were to hold is lost, and a page given to the entry later would
+// show a former owner's rows in their place. Steps that go on in it count it again.
 //
 // Two steps: the row step (one block, prefix sums over the rows, pushes) and
 // the fill step (every table entry, token and stack entry on its own). Order
@@ -190,8 +192,13 @@ __device__ void fill_step(const PageParams& p, uint32_t first, uint32_t stride) 
       slot[k] = -1;
       if (pos[k] >= 0) {  // pages that the row keeps are not written by this step
         const int j = pos[k] / p.block_size;
-        slot[k] = j < r[k].z ? p.table_in[(size_t)b[k] * p.max_blocks + j]
-                             : taken_page(p, r[k].w + j - r[k].z, total, free0);
+        if (j < r[k].z) {
+          slot[k] = p.table_in[(size_t)b[k] * p.max_blocks + j];
+          // the page that the row's first new token goes on in was missing in an earlier plan
+          if (slot[k] == -1 && pos[k] == r[k].x) atomicAdd(p.missing, 1);
+        } else {
+          slot[k] = taken_page(p, r[k].w + j - r[k].z, total, free0);
+        }
       }
     }
 #pragma unroll

@@ -37,9 +37,14 @@ def plan_pages(block_table, cached_lens, new_lens, free_blocks, free_count, bloc
     ``seq_lens`` ``[B]``, ``positions``, ``lengths`` (positions + 1, the
     indexer's key counts) and ``slots`` (cache rows, for ``append_kv``)
     ``[B, SQ]``, the stack ``free_blocks`` and ``free_count``, and ``missing``
-    ``[1]``, the pages that the stack could not give: their table entries and
-    the slots of their tokens are -1, so that they are neither written nor
-    read. Padding has position and slot -1 and length 0. Lengths out of range
+    ``[1]``, the pages that the new tokens lack: their table entries and the
+    slots of their tokens are -1, so that they are neither written nor read.
+    They are the ones that the stack could not give now, and those of earlier
+    steps (-1 in ``block_table``) in which new tokens go on: a page once missing
+    is not asked for again, since its earlier tokens are lost. Rows with a
+    position but no slot are the ones to ``reset`` and run again; their
+    ``seq_lens`` count the lost tokens (a caller that would rather wait for
+    pages keeps the inputs, without ``inplace``, and repeats the call). Padding has position and slot -1 and length 0. Lengths out of range
     are clamped (to ``[0, SQ]`` new tokens and to the table's room).
 
     New tensors are returned, unless ``inplace`` updates ``block_table``,

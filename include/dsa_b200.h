@@ -273,7 +273,10 @@ DSA_B200_API int dsa_rotary(const dsa_rotary_args_t* args, void* stream);
  *   slots          table_out[pos / block_size] * block_size + pos % block_size,
  *                  the row of dsa_append_kv; -1 for padding or without a page
  *   free_blocks_out, free_count_out   the stack afterwards
- *   missing        pages that were wanted and not there
+ *   missing        pages that the new tokens lack: wanted now and not there, or
+ *                  missing (-1 in block_table) since an earlier step that they go
+ *                  on from. A page once missing is not taken later: the row's
+ *                  earlier tokens are lost, and it has to be reset
  * In place: table_out, seq_lens, free_blocks_out and free_count_out may be
  * block_table, cached_lens, free_blocks and free_count. Counts and lengths out
  * of range are clamped; table entries outside [0, num_blocks) name no page. */

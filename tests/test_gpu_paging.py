@@ -128,6 +128,35 @@ def test_plan_steps_keep_every_page_once(cuda_lib):
             break
 
 
+@pytest.mark.parametrize("inplace", [False, True])
+def test_plan_after_a_missing_page(cuda_lib, inplace):
+    """A page that the stack could not give is reported by every step whose tokens would go on in it, also when the stack
+    has pages again; no other row is counted, the next page is given, and a reset row starts anew."""
+    i32 = dict(dtype=torch.int32, device="cuda")
+    table = torch.tensor([[5, -1, -1, -1], [6, 7, -1, -1], [-1, -1, -1, -1]], **i32)
+    lens, stack, count = torch.tensor([15, 20, 0], **i32), torch.zeros(8, **i32), torch.zeros(1, **i32)
+
+    def step(new, reset=None):
+        nonlocal table, lens, stack, count
+        r = None if reset is None else torch.tensor(reset, device="cuda")
+        plan = dsa_b200.plan_pages(table, lens, torch.tensor(new, **i32), stack, count, 16, 13, reset=r, inplace=inplace)
+        table, lens, stack, count = plan.block_table, plan.seq_lens, plan.free_blocks, plan.free_count
+        first = [[s for s, p in zip(*row) if p >= 0] for row in zip(plan.slots.tolist(), plan.positions.tolist())]
+        return int(plan.missing), first
+
+    assert step([2, 1, 0]) == (1, [[5 * 16 + 15, -1], [7 * 16 + 4], []])
+    stack[:4], count[:] = torch.tensor([1, 2, 3, 4], **i32), 4
+    assert step([1, 1, 0]) == (1, [[-1], [7 * 16 + 5], []])
+    assert step([0, 1, 0]) == (0, [[], [7 * 16 + 6], []])  # nothing goes on in it
+    # twelve tokens up to position 30, then the last of the missing page and the first of the next, which is there
+    assert step([13, 0, 0]) == (1, [[-1] * 13, [], []])
+    assert step([2, 0, 1]) == (1, [[-1, 4 * 16], [], [3 * 16]])
+    assert step([1, 0, 0]) == (0, [[4 * 16 + 1], [], []])
+    assert table.tolist() == [[5, -1, 4, -1], [6, 7, -1, -1], [3, -1, -1, -1]] and int(count) == 2
+    assert step([2, 0, 0], [True, False, False]) == (0, [[4 * 16, 4 * 16 + 1], [], []])
+    assert table.tolist()[0] == [4, -1, -1, -1] and stack[:int(count)].tolist() == [1, 2, 5]
+
+
 def _tokens(batch, queries, seed, parts=False):
     g = torch.Generator(device="cuda").manual_seed(seed)
     row = torch.randn((batch, queries, 1, 576), generator=g, device="cuda").bfloat16() * 3
