@@ -89,6 +89,8 @@ def plan_pages(block_table, cached_lens, new_lens, free_blocks, free_count, bloc
         free_count.data_ptr(), None if reset is None else reset.data_ptr(), table.data_ptr(), lens.data_ptr(),
         positions.data_ptr(), lengths.data_ptr(), slots.data_ptr(), stack.data_ptr(), count.data_ptr(),
         missing.data_ptr(), batch, queries, max_blocks, num_blocks, block_size, work.data_ptr(), 4 * words), index)
+    if inplace:
+        torch.autograd.graph.increment_version((table, lens, stack, count))
     return PagePlan(table, lens, positions, lengths, slots, stack, count, missing)
 
 
@@ -135,6 +137,7 @@ def _append(kv, k_rope, slots, latent, rope, fp8, rows, positions, inv_freq, lay
     api.enqueue("dsa_append_kv", _native.AppendKvArgs(
         kv.data_ptr(), k_rope.data_ptr(), slots.data_ptr(), pos_at, freq_at, *caches, batch, queries, rows,
         kv0, kv1, kr0, kr1, number, attention_factor), index)
+    torch.autograd.graph.increment_version((first,) if rope is None else (first, rope))
 
 
 def append_kv(kv, k_rope, slots, kv_cache, k_rope_cache, *, positions=None, inv_freq=None, layout="interleaved",

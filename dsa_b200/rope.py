@@ -146,7 +146,8 @@ def rotary(x, positions, inv_freq, *, layout="interleaved", start=0, attention_f
     copied. ``inverse`` turns back by ``-t`` (still times ``f``).
 
     Returns a new contiguous tensor, or ``out`` (same shape and type; ``x``
-    itself for an update in place). Without ``out`` the call is differentiable
+    itself for an update in place; autograd learns of the write, as of torch's
+    own in-place operations). Without ``out`` the call is differentiable
     in ``x``; the gradient is one launch of the same kernel. Angles are reduced
     exactly (64-bit fractions of a turn), cosines and products are FP32, rounded
     once to the type of ``x``; frequencies and the factor are finite.
@@ -180,7 +181,9 @@ def rotary(x, positions, inv_freq, *, layout="interleaved", start=0, attention_f
     if not same and device.type == "cuda" and out.untyped_storage().data_ptr() == x.untyped_storage().data_ptr() \
             and not _apart(x, out):
         raise ValueError("out must be x itself or not overlap it")
-    return _launch(x, positions, inv_freq, out, number, start, attention_factor, inverse)
+    _launch(x, positions, inv_freq, out, number, start, attention_factor, inverse)
+    torch.autograd.graph.increment_version(out)
+    return out
 
 
 def _apart(a, b):

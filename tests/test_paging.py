@@ -61,3 +61,32 @@ def test_append_refusals(monkeypatch):
     for cache, why in [(t(9, 16, 1, 655, dtype=torch.uint8), "need cache"), (t(9, 16, 1, 656, dtype=torch.int8), "uint8")]:
         with pytest.raises(ValueError, match=why):
             dsa_b200.append_kv_fp8(kv, kr, slots, cache)
+
+
+def test_writes_tell_autograd(monkeypatch):
+    """Every tensor of the caller that a call writes counts as modified in place; the ones that it reads do not."""
+    monkeypatch.setattr(api, "DEVICE_TYPE", "cpu")
+    monkeypatch.setattr(api, "enqueue", lambda *args: None)
+
+    def z(*shape, dtype=torch.int32):
+        return torch.zeros(shape, dtype=dtype)
+
+    table, cached, new, stack, count = z(4, 8), z(4), z(4), z(32), z(1)
+    for inplace in (False, True):
+        plan = dsa_b200.plan_pages(table, cached, new, stack, count, 16, 5, inplace=inplace)
+        assert [t._version for t in (table, cached, new, stack, count)] == [int(inplace)] * 2 + [0] + [int(inplace)] * 2
+    assert plan.block_table is table
+    bf = torch.bfloat16
+    kv, kr, slots = z(2, 3, 1, 512, dtype=bf), z(2, 3, 1, 64, dtype=bf), z(2, 3)
+    pool, rope, rows = z(9, 16, 1, 512, dtype=bf), z(9, 16, 1, 64, dtype=bf), z(9, 16, 1, 656, dtype=torch.uint8)
+    dsa_b200.append_kv(kv, kr, slots, pool, rope)
+    dsa_b200.append_kv_fp8(kv, kr, slots, rows)
+    assert [t._version for t in (kv, kr, slots, pool, rope, rows)] == [0, 0, 0, 1, 1, 1]
+    w = torch.ones(512, dtype=bf, requires_grad=True)
+    y = pool * w
+    dsa_b200.append_kv(kv, kr, slots, pool, rope)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    with torch.inference_mode():
+        pool, rope = z(9, 16, 1, 512, dtype=bf), z(9, 16, 1, 64, dtype=bf)
+    dsa_b200.append_kv(kv, kr, slots, pool, rope)  # have no version

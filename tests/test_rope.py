@@ -64,3 +64,21 @@ def test_rotary_refusals(monkeypatch):
         dsa_b200.rotary(torch.empty(2, 3, 4, 64, dtype=torch.bfloat16), pos, freq)
     with pytest.raises(ValueError, match="autograd"):
         dsa_b200.rotary(t(2, 3, 4, 64).requires_grad_(), pos, t(32, dtype=torch.float64), out=t(2, 3, 4, 64))
+
+
+def test_out_tells_autograd(monkeypatch):
+    """A tensor that was saved for a backward pass and then turned in place: torch's error, no gradient of other values."""
+    monkeypatch.setattr(api, "DEVICE_TYPE", "cpu")
+    monkeypatch.setattr(api, "enqueue", lambda *args: None)
+    x, w = torch.randn(2, 3, 4, 64), torch.ones(64, requires_grad=True)
+    pos, freq = torch.zeros(2, 3, dtype=torch.int32), dsa_b200.rotary_frequencies(64)
+    y, part = x * w, x[:, :, :2]
+    assert dsa_b200.rotary(part, pos, freq, out=part) is part and x._version == 1  # a view shares its base's
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    before = x._version
+    dsa_b200.rotary(x, pos, freq)
+    assert x._version == before
+    with torch.inference_mode():
+        z = torch.zeros(2, 3, 4, 64)
+    dsa_b200.rotary(z, pos, freq, out=z)  # has no version
