@@ -11,6 +11,7 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native, api
 
@@ -110,15 +111,37 @@ def _launch(x, positions, inv_freq, out, number, start, factor, inverse):
     return out
 
 
+def _followed(x):
+    """Whether autograd follows what becomes of ``x``: backwards, or forwards as the primal of a dual tensor."""
+    return ((x.requires_grad and torch.is_grad_enabled())
+            or (forward_ad._current_level >= 0 and forward_ad.unpack_dual(x).tangent is not None))
+
+
+def _turn(x, positions, inv_freq, number, start, factor, inverse):
+    """The rotation of ``x`` as a new tensor, with its derivatives where autograd follows it."""
+    if _followed(x):
+        return _Rotary.apply(x, (positions, inv_freq, number, start, factor, inverse))
+    return _launch(x, positions, inv_freq, _rows_like(x), number, start, factor, inverse)
+
+
 class _Rotary(torch.autograd.Function):
-    """The rotation is linear with an orthogonal matrix times the factor: its gradient is the inverse rotation."""
+    """The rotation is linear with an orthogonal matrix times the factor: its gradient is the inverse rotation, its
+    forward-mode derivative the rotation itself."""
 
     @staticmethod
     def forward(ctx, x, turn):  # one argument beside x: every further one costs the engine host time
         positions, inv_freq, *how = turn
         ctx.save_for_backward(positions, inv_freq)
         ctx.how = how
+        ctx.turn = turn if forward_ad._current_level >= 0 else None  # for jvp, which follows at once
         return _launch(x, positions, inv_freq, _rows_like(x), *how)
+
+    @staticmethod
+    def jvp(ctx, tangent, _):
+        turn, ctx.turn = ctx.turn, None
+        if tangent._is_zerotensor():  # no memory behind it
+            return torch.zeros(tangent.shape, dtype=tangent.dtype, device=tangent.device)
+        return _turn(tangent if tangent.stride(-1) == 1 else tangent.contiguous(), *turn)
 
     @staticmethod
     def backward(ctx, grad):
@@ -126,9 +149,7 @@ class _Rotary(torch.autograd.Function):
         number, start, factor, inverse = ctx.how
         if grad.stride(-1) != 1:
             grad = grad.contiguous()
-        if torch.is_grad_enabled():  # a graph of the gradient is wanted
-            return _Rotary.apply(grad, (positions, inv_freq, number, start, factor, not inverse)), None
-        return _launch(grad, positions, inv_freq, _rows_like(grad), number, start, factor, not inverse), None
+        return _turn(grad, positions, inv_freq, number, start, factor, not inverse), None
 
 
 def rotary(x, positions, inv_freq, *, layout="interleaved", start=0, attention_factor=1.0, inverse=False, out=None):
@@ -148,7 +169,8 @@ def rotary(x, positions, inv_freq, *, layout="interleaved", start=0, attention_f
     Returns a new contiguous tensor, or ``out`` (same shape and type; ``x``
     itself for an update in place; autograd learns of the write, as of torch's
     own in-place operations). Without ``out`` the call is differentiable
-    in ``x``; the gradient is one launch of the same kernel. Angles are reduced
+    in ``x``, backwards and in forward mode; a derivative is one launch of the
+    same kernel. Angles are reduced
     exactly (64-bit fractions of a turn), cosines and products are FP32, rounded
     once to the type of ``x``; frequencies and the factor are finite.
     """
@@ -170,12 +192,10 @@ def rotary(x, positions, inv_freq, *, layout="interleaved", start=0, attention_f
         raise ValueError("the last dimension of x must be contiguous")
     inverse = bool(inverse)
     if out is None:
-        if x.requires_grad and torch.is_grad_enabled():
-            return _Rotary.apply(x, (positions, inv_freq, number, start, attention_factor, inverse))
-        return _launch(x, positions, inv_freq, _rows_like(x), number, start, attention_factor, inverse)
+        return _turn(x, positions, inv_freq, number, start, attention_factor, inverse)
     if out.shape != x.shape or out.dtype != x.dtype or out.device != device or out.stride(-1) != 1 or _overlaps_itself(out):
         raise ValueError("out must have the shape, type and device of x and rows that do not overlap")
-    if torch.is_grad_enabled() and (x.requires_grad or out.requires_grad):
+    if _followed(x) or _followed(out):
         raise ValueError("out does not take part in autograd: leave it out, or call under torch.no_grad()")
     same = out.data_ptr() == x.data_ptr() and all(n == 1 or a == b for n, a, b in zip(x.shape, x.stride(), out.stride()))
     if not same and device.type == "cuda" and out.untyped_storage().data_ptr() == x.untyped_storage().data_ptr() \

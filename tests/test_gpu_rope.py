@@ -138,6 +138,25 @@ def test_second_derivative(cuda_lib):
     _check(gg, v, pos, freq)
 
 
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+def test_forward_mode(cuda_lib, layout):
+    """The tangent is turned as a tensor of its own would be, contiguous or not, and zero where it is known to be zero."""
+    x, pos = _make((2, 5, 3, 80), torch.float32, 9, 1000)
+    t = torch.randn_like(x)
+    freq = dsa_b200.rotary_frequencies(32, device="cuda")
+
+    def turn(x):
+        return dsa_b200.rotary(x, pos, freq, layout=layout, start=16, attention_factor=0.75)
+
+    with torch.autograd.forward_ad.dual_level():
+        for tangent in (t, t.permute(3, 2, 1, 0).contiguous().permute(3, 2, 1, 0)):
+            y = torch.autograd.forward_ad.unpack_dual(turn(torch.autograd.forward_ad.make_dual(x, tangent)))
+            assert torch.equal(y.primal, turn(x)) and torch.equal(y.tangent, turn(t))
+        zero = torch._efficientzerotensor(x.shape, device="cuda")
+        y = torch.autograd.forward_ad.unpack_dual(turn(torch.autograd.forward_ad.make_dual(x, zero)))
+        assert torch.equal(y.primal, turn(x)) and (y.tangent is None or not bool(y.tangent.any()))
+
+
 def test_captured_with_new_positions(cuda_lib):
     x, pos = _make((4, 1, 16, 64), torch.bfloat16, 1)
     freq = dsa_b200.rotary_frequencies(64, device="cuda")

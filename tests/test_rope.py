@@ -3,9 +3,10 @@ import math
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import dsa_b200
-from dsa_b200 import api
+from dsa_b200 import api, rope
 
 
 def test_frequencies():
@@ -82,3 +83,41 @@ def test_out_tells_autograd(monkeypatch):
     with torch.inference_mode():
         z = torch.zeros(2, 3, 4, 64)
     dsa_b200.rotary(z, pos, freq, out=z)  # has no version
+
+
+def _plain_launch(x, positions, inv_freq, out, number, start, factor, inverse):
+    """The kernel's map, interleaved pairs of whole rows."""
+    t = (positions.double()[..., None, None] * inv_freq).to(x.dtype) * (-1 if inverse else 1)
+    a, b = x.detach()[..., 0::2], x.detach()[..., 1::2]
+    return out.copy_(factor * torch.stack((a * t.cos() - b * t.sin(), b * t.cos() + a * t.sin()), -1).flatten(-2))
+
+
+def test_forward_mode(monkeypatch):
+    """The tangent is turned as the primal is, alone, with a graph of the tangent, and through the backward pass."""
+    monkeypatch.setattr(api, "DEVICE_TYPE", "cpu")
+    monkeypatch.setattr(rope, "_launch", _plain_launch)
+    x, t, g = torch.randn(3, 2, 3, 4, 64).unbind(0)
+    pos, freq = torch.arange(6, dtype=torch.int32).reshape(2, 3), dsa_b200.rotary_frequencies(64)
+
+    def turn(x, **kw):
+        return dsa_b200.rotary(x, pos, freq, attention_factor=1.5, **kw)
+
+    with forward_ad.dual_level():
+        for tangent in (t, t[..., :1].expand(2, 3, 4, 64), t.transpose(2, 3).contiguous().transpose(2, 3)):
+            y = forward_ad.unpack_dual(turn(forward_ad.make_dual(x, tangent)))
+            assert torch.equal(y.primal, turn(x)) and torch.equal(y.tangent, turn(tangent.contiguous()))
+        with torch.no_grad():
+            assert torch.equal(forward_ad.unpack_dual(turn(forward_ad.make_dual(x, t))).tangent, turn(t))
+        assert forward_ad.unpack_dual(turn(x)).tangent is None
+        with pytest.raises(ValueError, match="autograd"), torch.no_grad():
+            dual = forward_ad.make_dual(x, t)
+            turn(dual, out=dual)
+        # the tangent's own graph
+        t.requires_grad_()
+        dot = forward_ad.unpack_dual(turn(forward_ad.make_dual(x, t))).tangent
+        (gt,) = torch.autograd.grad(dot, t, g)
+        assert torch.equal(gt, turn(g, inverse=True))
+        # the gradient's tangent: that of its own input
+        leaf = x.clone().requires_grad_()
+        (gx,) = torch.autograd.grad(turn(leaf), leaf, forward_ad.make_dual(g, t.detach()))
+        assert torch.equal(forward_ad.unpack_dual(gx).tangent, turn(t.detach(), inverse=True))
