@@ -16,7 +16,7 @@ from collections import namedtuple
 import torch
 
 from . import _native, api
-from .rope import _check_rope
+from .rope import _check_rope, _followed
 
 PagePlan = namedtuple("PagePlan", "block_table seq_lens positions lengths slots free_blocks free_count missing")
 
@@ -117,6 +117,8 @@ def _append(kv, k_rope, slots, latent, rope, fp8, rows, positions, inv_freq, lay
         raise ValueError("all inputs must be on the same CUDA device")
     if not slots.is_contiguous() or not first.is_contiguous() or (rope is not None and not rope.is_contiguous()):
         raise ValueError("slots and the cache must be contiguous")
+    if _followed(kv) or _followed(k_rope) or _followed(first) or (rope is not None and _followed(rope)):
+        raise ValueError("appends have no gradient: call them under torch.no_grad() or detach kv, k_rope and the cache")
     if inv_freq is not None and positions is not None:
         number = _check_rope(positions, inv_freq, layout, attention_factor, lead, index)
         if positions.dtype is not int32 or not positions.is_contiguous() or inv_freq.shape[0] != 32:

@@ -12,6 +12,7 @@ from __future__ import annotations
 import torch
 
 from . import _native, api
+from .rope import _followed
 
 WORKSPACE_BUDGET = 1 << 31  # bytes of FP32 partials per library call
 _AUTO = _native.Launch()  # family 0: the library's choice
@@ -33,7 +34,8 @@ def forward_shared_prefix(q, prefix_kv, q_rope, prefix_k_rope, kv=None, k_rope=N
     Returns ``(output, softmax_max, softmax_sum)`` as ``forward`` does, over
     both sets of keys: indices outside ``[0, L)`` are masked, duplicates keep
     their repeated weight, a row without any key gets output 0, maximum -inf
-    and sum 0, one with a NaN score NaN, -inf and NaN. Asynchronous on the
+    and sum 0, one with a NaN score NaN, -inf and NaN. The call has no gradient
+    and refuses inputs that autograd follows. Asynchronous on the
     current stream; partials are FP32, in pieces of whole queries that keep
     them under ``WORKSPACE_BUDGET`` bytes.
     """
@@ -66,6 +68,8 @@ def forward_shared_prefix(q, prefix_kv, q_rope, prefix_k_rope, kv=None, k_rope=N
             raise ValueError("q, q_rope, the prefix and kv/k_rope must be bfloat16, indices and prefix_len int32")
         if t.get_device() != index or not t.is_contiguous():
             raise ValueError("all inputs must be contiguous and on the same CUDA device")
+        if _followed(t):
+            raise ValueError("forward_shared_prefix has no gradient: call it under torch.no_grad() or detach its inputs")
     if prefix_len is not None and prefix_len.numel() != 1:
         raise ValueError("prefix_len must be an int32 tensor of one element")
     for t in (indices, prefix_len):

@@ -90,3 +90,22 @@ def test_writes_tell_autograd(monkeypatch):
     with torch.inference_mode():
         pool, rope = z(9, 16, 1, 512, dtype=bf), z(9, 16, 1, 64, dtype=bf)
     dsa_b200.append_kv(kv, kr, slots, pool, rope)  # have no version
+
+
+def test_append_refuses_gradients(monkeypatch):
+    """No gradient goes through a cache: values and caches that autograd follows are refused outside torch.no_grad()."""
+    monkeypatch.setattr(api, "DEVICE_TYPE", "cpu")
+    monkeypatch.setattr(api, "enqueue", lambda *args: None)
+    bf = torch.bfloat16
+    plain = [torch.zeros(s, dtype=bf) for s in ((2, 3, 1, 512), (2, 3, 1, 64), (9, 16, 1, 512), (9, 16, 1, 64))]
+    slots, rows = torch.zeros((2, 3), dtype=torch.int32), torch.zeros((9, 16, 1, 656), dtype=torch.uint8)
+    for k in range(4):
+        kv, kr, pool, rope = [t.clone().requires_grad_() if i == k else t for i, t in enumerate(plain)]
+        with pytest.raises(ValueError, match="no gradient"):
+            dsa_b200.append_kv(kv, kr, slots, pool, rope)
+        if k < 2:
+            with pytest.raises(ValueError, match="no gradient"):
+                dsa_b200.append_kv_fp8(kv, kr, slots, rows)
+        with torch.no_grad():
+            dsa_b200.append_kv(kv, kr, slots, pool, rope)
+            dsa_b200.append_kv_fp8(kv, kr, slots, rows)

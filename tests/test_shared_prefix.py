@@ -67,3 +67,23 @@ def test_plan():
     assert lib.dsa_fwd_prefix_plan(a, px, None) == _native.STATUS_BAD_ARGUMENT
     a.heads = 24
     assert lib.dsa_fwd_prefix_plan(a, px, plan) == _native.STATUS_BAD_ARGUMENT
+
+
+def test_gradients_are_refused(monkeypatch):
+    """The outputs have no graph: inputs that autograd follows, in either mode, are refused, not cut off."""
+    monkeypatch.setattr(api, "DEVICE_TYPE", "cpu")
+    monkeypatch.setattr(api, "enqueue", lambda *args: None)
+    monkeypatch.setattr(api, "_status_words", {})
+    shapes = (2, 3, 16, 512), (1, 50, 1, 512), (2, 3, 16, 64), (1, 50, 1, 64), (2, 9, 1, 512), (2, 9, 1, 64)
+    ids = torch.zeros((2, 3, 1, 5), dtype=torch.int32)
+    plain = [torch.zeros(s, dtype=torch.bfloat16) for s in shapes]
+    for k in range(6):
+        args = [t.clone().requires_grad_() if i == k else t for i, t in enumerate(plain)]
+        with pytest.raises(ValueError, match="no gradient"):
+            dsa_b200.forward_shared_prefix(*args, ids)
+        with torch.no_grad():
+            dsa_b200.forward_shared_prefix(*args, ids)
+        dsa_b200.forward_shared_prefix(*(t.detach() for t in args), ids)
+        with torch.autograd.forward_ad.dual_level(), pytest.raises(ValueError, match="no gradient"):
+            dual = torch.autograd.forward_ad.make_dual(plain[k], plain[k])
+            dsa_b200.forward_shared_prefix(*(dual if i == k else t for i, t in enumerate(plain)), ids)
