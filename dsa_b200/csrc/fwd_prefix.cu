@@ -32,10 +32,15 @@
 //
 // P rounds the weights to BF16 for the MMA; the row sum adds them before the
 // rounding, in FP32 (as every other family here). A score is 36 accumulations
-// of the MMA, each cut to FP32: on random data it ends 5.6e-7 of itself too
-// near to zero on average (so does the pair family's), and is exact where the
-// products' sums are. Nothing corrects for it: the loss depends on the data,
-// and the own keys' scores, which share the softmax, lose theirs alike.
+// of the MMA, each cut to FP32: it is exact where the sums of the products are,
+// within 36 * 2^-23 of its partial sums' size anywhere, and on random data
+// 5.6e-7 of itself too near to zero on average (softmax_sum then 1.8e-6 too
+// large; an FP32 product of torch's is 2e-7 and 7e-7 off), as in the pair
+// family. Nothing corrects for it: the loss depends on the data, and the own
+// keys' scores, which share the softmax, lose theirs alike. Two sums a score
+// (dims 0-255, the rest; three S buffers fit the TMEM) halve the loss, 7.7e-7
+// on the sum, but the second buffer's reads and its turn-around take 13 % of
+// 4096 rows over 32003 keys (201 -> 228 us) and 11 % of 1024 over 32768.
 //
 // Roles (12 warps; the MMAs of a pair are issued by its first CTA): score CTA
 // 0 TMA, 1 and 3 QK issuers of the even and the odd tiles, in turn (an issuer
@@ -1001,7 +1006,9 @@ cudaError_t launch_fwd_prefix(const PrefixParams& p, const void* kv, const void*
 cudaError_t launch_prefix_join(const JoinParams& p, cudaStream_t stream) {
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;  // its start overlaps the end of the kernel before it
+  // Its blocks wait themselves: beside the prefix kernel where there are no own
+  // keys; the own keys' kernel lets them start only at its own end.
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   if (p.split + p.own_split > kJoinMaxParts) return cudaErrorInvalidValue;
   cfg.gridDim = dim3((unsigned)((p.rows + 31) / 32), kDimLatent / (8 * kJoinWarps), 1);

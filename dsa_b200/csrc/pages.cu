@@ -15,8 +15,8 @@
 // the fill step (every table entry, token and stack entry on its own). Order
 // is fixed by prefix sums, so equal inputs give equal plans. The
 // work is a few bytes per entry: latency bounds it, not bandwidth. They
-// are two launches, the second started early and waiting for the first on the
-// GPU; one launch of an eight-block cluster with its barrier between the steps
+// are two launches, the second a programmatic one, which waits for the first on
+// the GPU (the row step lets it start only at its own end); one launch of an eight-block cluster with its barrier between the steps
 // was no faster for small plans (6.2 us) and slower for others (64 rows of 1024
 // pages 11.8 against 9.3 us).
 #include "serving.cuh"
@@ -245,7 +245,7 @@ cudaError_t launch_plan_pages(const PageParams& p, cudaStream_t stream) {
   if (blocks > 148 * 8) blocks = 148 * 8;
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;  // its start overlaps the end of the row step
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;  // plan_fill_kernel waits itself
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.gridDim = dim3((unsigned)blocks, 1, 1);
   cfg.blockDim = dim3(256, 1, 1);

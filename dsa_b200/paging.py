@@ -154,7 +154,9 @@ def append_kv(kv, k_rope, slots, kv_cache, k_rope_cache, *, positions=None, inv_
     nothing (padding is -1); the other rows keep what they hold. Slots of one
     call must be distinct (those of a plan are). With ``positions`` (int32
     ``[B, S]``) and ``inv_freq`` (FP64 ``[32]``) ``k_rope`` is turned first, as
-    by ``rotary``; without them it is stored as given.
+    by ``rotary``; without them it is stored as given. ``kv`` and ``k_rope``
+    share no memory with the cache. No gradient goes through a cache: tensors
+    that autograd follows are refused.
     """
     shape = kv_cache.shape
     if len(shape) != 4 or shape[2] != 1 or shape[3] != 512 or not shape[0] or not shape[1]:

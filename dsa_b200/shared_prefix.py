@@ -6,6 +6,12 @@ same leading keys. ``forward`` would gather those keys again for every query;
 dense product and joins the result with each query's own selected keys. The
 reference has no such call: its forward takes every key through a query's
 index row (dsa/api.py:76-132).
+
+The prefix is attended to in full, not by selection. That is dense MLA
+attention (a model without an indexer, or its dense layers and warm-up), and
+sparse attention as long as the whole prefix is among the selected keys, that
+is up to the indexer's top-k. Beyond it a model with an indexer lets prefix and
+own keys compete for the top-k: ``indexer_topk`` and ``forward`` over both.
 """
 from __future__ import annotations
 
@@ -25,7 +31,8 @@ def forward_shared_prefix(q, prefix_kv, q_rope, prefix_k_rope, kv=None, k_rope=N
     ``prefix_kv`` BF16 ``[1, P, 1, 512]`` and ``prefix_k_rope`` ``[1, P, 1, 64]``
     are attended to by every query in full (``prefix_len``, an int32 ``[1]``
     tensor on the device, limits them to the first ``prefix_len`` rows; the
-    rows behind may hold anything). ``kv`` ``[B, L, 1, 512]``, ``k_rope``
+    rows behind may hold anything. The launch is planned for all ``P`` rows: a
+    buffer filled in small part is better cut to size where the host knows it). ``kv`` ``[B, L, 1, 512]``, ``k_rope``
     ``[B, L, 1, 64]`` and ``indices`` int32 ``[B, SQ, 1, K]`` are ``forward``'s
     for the keys of each batch row itself; without them the prefix is all
     there is. ``q`` ``[B, SQ, H, 512]`` and ``q_rope`` ``[B, SQ, H, 64]``, H a

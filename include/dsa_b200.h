@@ -313,7 +313,7 @@ DSA_B200_API int dsa_plan_pages(const dsa_plan_pages_args_t* args, void* stream)
  * block of zeros), else kv_cache / k_rope_cache are the BF16 rows of
  * dsa_sparse_mla_fwd(_paged). A slot outside [0, rows) writes nothing. Slots
  * of one call are distinct; of two tokens with one slot either may win, or
- * parts of both. */
+ * parts of both. kv and k_rope share no memory with the cache. */
 typedef struct dsa_append_kv_args {
   const void* kv;            /* BF16 [batch, queries, 512], last dim contiguous */
   const void* k_rope;        /* BF16 [batch, queries, 64], last dim contiguous */
