@@ -13,12 +13,12 @@
 //
 // Two steps: the row step (one block, prefix sums over the rows, pushes) and
 // the fill step (every table entry, token and stack entry on its own). Order
-// is fixed by prefix sums, so equal inputs give equal plans. The
-// work is a few bytes per entry: latency bounds it, not bandwidth. They
-// are two launches, the second a programmatic one, which waits for the first on
-// the GPU (the row step lets it start only at its own end); one launch of an eight-block cluster with its barrier between the steps
-// was no faster for small plans (6.2 us) and slower for others (64 rows of 1024
-// pages 11.8 against 9.3 us).
+// is fixed by prefix sums, so equal inputs give equal plans. The work is a few
+// bytes per entry: latency bounds it, not bandwidth. They are two launches, the
+// second a programmatic one, which waits for the first on the GPU (the row step
+// lets it start only at its own end); one launch of an eight-block cluster with
+// its barrier between the steps was no faster for small plans (6.2 us) and
+// slower for others (64 rows of 1024 pages 11.8 against 9.3 us).
 #include "serving.cuh"
 
 namespace dsa {

@@ -44,8 +44,9 @@ def plan_pages(block_table, cached_lens, new_lens, free_blocks, free_count, bloc
     is not asked for again, since its earlier tokens are lost. Rows with a
     position but no slot are the ones to ``reset`` and run again; their
     ``seq_lens`` count the lost tokens (a caller that would rather wait for
-    pages keeps the inputs, without ``inplace``, and repeats the call). Padding has position and slot -1 and length 0. Lengths out of range
-    are clamped (to ``[0, SQ]`` new tokens and to the table's room).
+    pages keeps the inputs, without ``inplace``, and repeats the call). Padding
+    has position and slot -1 and length 0. Lengths out of range are clamped (to
+    ``[0, SQ]`` new tokens and to the table's room).
 
     New tensors are returned, unless ``inplace`` updates ``block_table``,
     ``cached_lens`` (to ``seq_lens``), ``free_blocks`` and ``free_count``; the

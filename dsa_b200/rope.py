@@ -168,11 +168,11 @@ def rotary(x, positions, inv_freq, *, layout="interleaved", start=0, attention_f
 
     Returns a new contiguous tensor, or ``out`` (same shape and type; ``x``
     itself for an update in place; autograd learns of the write, as of torch's
-    own in-place operations). Without ``out`` the call is differentiable
-    in ``x``, backwards and in forward mode; a derivative is one launch of the
-    same kernel. Angles are reduced
-    exactly (64-bit fractions of a turn), cosines and products are FP32, rounded
-    once to the type of ``x``; frequencies and the factor are finite.
+    own in-place operations). Without ``out`` the call is differentiable in
+    ``x``, backwards and in forward mode; a derivative is one launch of the same
+    kernel. Angles are reduced exactly (64-bit fractions of a turn), cosines and
+    products are FP32, rounded once to the type of ``x``; frequencies and the
+    factor are finite.
     """
     shape = x.shape
     if len(shape) not in (3, 4) or 0 in shape:

@@ -31,11 +31,12 @@ def forward_shared_prefix(q, prefix_kv, q_rope, prefix_k_rope, kv=None, k_rope=N
     ``prefix_kv`` BF16 ``[1, P, 1, 512]`` and ``prefix_k_rope`` ``[1, P, 1, 64]``
     are attended to by every query in full (``prefix_len``, an int32 ``[1]``
     tensor on the device, limits them to the first ``prefix_len`` rows; the
-    rows behind may hold anything. The launch is planned for all ``P`` rows: a
-    buffer filled in small part is better cut to size where the host knows it). ``kv`` ``[B, L, 1, 512]``, ``k_rope``
-    ``[B, L, 1, 64]`` and ``indices`` int32 ``[B, SQ, 1, K]`` are ``forward``'s
-    for the keys of each batch row itself; without them the prefix is all
-    there is. ``q`` ``[B, SQ, H, 512]`` and ``q_rope`` ``[B, SQ, H, 64]``, H a
+    rows behind may hold anything; the launch is planned for all ``P`` rows, so
+    a buffer filled in small part is better cut to size where the host knows
+    it). ``kv`` ``[B, L, 1, 512]``, ``k_rope`` ``[B, L, 1, 64]`` and ``indices``
+    int32 ``[B, SQ, 1, K]`` are ``forward``'s for the keys of each batch row
+    itself (rows that no valid index names may hold anything too); without them
+    the prefix is all there is. ``q`` ``[B, SQ, H, 512]`` and ``q_rope`` ``[B, SQ, H, 64]``, H a
     multiple of 16, are turned already, at positions behind the prefix.
 
     Returns ``(output, softmax_max, softmax_sum)`` as ``forward`` does, over
